@@ -212,9 +212,13 @@ def run(state):
         if kind == "select":
             return ops.beam_select(s["logits"], s["scores"], s["count"])
         if kind == "pages":
-            ops.reorder_pages(s["pages"], s["table"], s["parents"], s["first"], s["lengths"])
+            if "set" not in s:                         # a program makes it once, with its cache
+                s["set"] = ops.PageSet(s["pages"])
+            ops.reorder_pages(s["set"], s["table"], s["parents"], s["first"], s["lengths"])
             return s["all"].view(torch.int16 if s["all"].element_size() == 2 else torch.int32)
-        ops.reorder_slots(s["states"], s["slots"], s["parents"])
+        if "set" not in s:
+            s["set"] = ops.SlotSet(s["states"])
+        ops.reorder_slots(s["set"], s["slots"], s["parents"])
         return s["all"].view(torch.int32)
 
     if kind == "quantize":
