@@ -1,0 +1,172 @@
+// Beams that go on from one another: row r of a group of `width` rows takes over what row parent[r] of its group holds, all rows
+// at once (a row may be the parent of others and have another parent itself).  Two forms of what a row holds: positions of paged
+// tensors, reached through a block table, and slots of fixed-size states.
+//
+// A thread owns one place (16 bytes of one position's row, or of one state) in all rows of a group: it reads the parents'
+// values of every row that moves, and writes them after the last read.  So no second copy is needed whatever the parents are,
+// and nothing is synchronised.  All tensors of a call are handled by one launch.
+#include "common.cuh"
+
+namespace {
+
+constexpr int RE_TENSORS = 128, RE_MAX_WIDTH = 32, RE_THREADS = 256;
+
+struct PageTensors {                       // [heads, pages, page_size, a row of row_bytes]
+    char* base[RE_TENSORS];
+    int heads[RE_TENSORS], pages[RE_TENSORS], row_bytes[RE_TENSORS];
+};
+struct SlotTensors {                       // [slots, slot_bytes]
+    char* base[RE_TENSORS];
+    long long bytes[RE_TENSORS];
+    int slots[RE_TENSORS];
+};
+
+// The group's parents; a parent outside the group counts as the row itself, which stays.
+__device__ __forceinline__ int parent_of(const int* parents, int group, int width, int b) {
+    const int p = parents[group * width + b];
+    return (unsigned)p < (unsigned)width ? p : b;
+}
+
+// grid (blocks along the places, tensors, groups); V: what a thread moves at a time; W: the most rows of a group.
+template <typename V, int W>
+__global__ void __launch_bounds__(RE_THREADS) reorder_pages_kernel(const __grid_constant__ PageTensors t, const int* table, int blocks, int page_size, const int* parents,
+                                                                   const int* first, const int* lengths, int width) {
+    pdl_enter();
+    __shared__ int par[RE_MAX_WIDTH], from[RE_MAX_WIDTH], to[RE_MAX_WIDTH];
+    const int group = blockIdx.z, row0 = group * width;
+    if (threadIdx.x < width) {
+        const int b = threadIdx.x, p = parent_of(parents, group, width, b);
+        par[b] = p, from[b] = max(first[row0 + b], 0), to[b] = p == b ? 0 : (int)min((long long)lengths[row0 + p], (long long)blocks * page_size);
+    }
+    __syncthreads();
+    int lo = 0x7fffffff, hi = 0;
+    for (int b = 0; b < width; ++b)
+        if (from[b] < to[b]) lo = min(lo, from[b]), hi = max(hi, to[b]);
+    if (lo >= hi) return;
+    char* base = t.base[blockIdx.y];
+    const int heads = t.heads[blockIdx.y], pages = t.pages[blockIdx.y], vecs = t.row_bytes[blockIdx.y] / (int)sizeof(V);
+    const long long page_bytes = (long long)page_size * t.row_bytes[blockIdx.y];
+    const long long places = (long long)(hi - lo) * heads * vecs;
+    for (long long i = (long long)blockIdx.x * RE_THREADS + threadIdx.x; i < places; i += (long long)gridDim.x * RE_THREADS) {
+        const int vec = (int)(i % vecs), head = (int)(i / vecs % heads), pos = lo + (int)(i / vecs / heads);
+        const int block = pos / page_size;
+        const long long in_page = (long long)(pos % page_size) * t.row_bytes[blockIdx.y] + (long long)vec * sizeof(V);
+        auto where = [&](int b) -> V* {
+            const int page = table[(long long)(row0 + b) * blocks + block];
+            return (unsigned)page < (unsigned)pages ? (V*)(base + ((long long)head * pages + page) * page_bytes + in_page) : nullptr;
+        };
+        V held[W];
+        V* dst[W];
+#pragma unroll
+        for (int b = 0; b < W; ++b) {
+            dst[b] = nullptr;
+            if (b < width && pos >= from[b] && pos < to[b]) {
+                const V* src = where(par[b]);
+                if (src) held[b] = *src, dst[b] = where(b);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < W; ++b)
+            if (dst[b]) *dst[b] = held[b];
+    }
+}
+
+template <typename V, int W>
+__global__ void __launch_bounds__(RE_THREADS) reorder_slots_kernel(const __grid_constant__ SlotTensors t, const int* slots, const int* parents, int width) {
+    pdl_enter();
+    __shared__ int par[RE_MAX_WIDTH], slot[RE_MAX_WIDTH];
+    const int group = blockIdx.z;
+    if (threadIdx.x < width) {
+        const int b = threadIdx.x, s = slots[group * width + b];
+        par[b] = parent_of(parents, group, width, b), slot[b] = (unsigned)s < (unsigned)t.slots[blockIdx.y] ? s : -1;
+    }
+    __syncthreads();
+    char* base = t.base[blockIdx.y];
+    const long long bytes = t.bytes[blockIdx.y], places = bytes / (long long)sizeof(V);
+    for (long long i = (long long)blockIdx.x * RE_THREADS + threadIdx.x; i < places; i += (long long)gridDim.x * RE_THREADS) {
+        V held[W];
+        bool moves[W];
+#pragma unroll
+        for (int b = 0; b < W; ++b) {
+            moves[b] = b < width && par[b] != b && slot[b] >= 0 && slot[par[b]] >= 0;
+            if (moves[b]) held[b] = *(const V*)(base + slot[par[b]] * bytes + i * (long long)sizeof(V));
+        }
+#pragma unroll
+        for (int b = 0; b < W; ++b)
+            if (moves[b]) *(V*)(base + slot[b] * bytes + i * (long long)sizeof(V)) = held[b];
+    }
+}
+
+// The widest of 16, 4 and 1 bytes that divides every address and size or'ed into `all`.
+int vector_bytes(unsigned long long all) { return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1; }
+
+template <typename V>
+void launch_pages(const PageTensors& t, int n, int groups, int width, int blocks_x, const int* table, int blocks, int page_size, const int* parents, const int* first,
+                  const int* lengths, cudaStream_t st) {
+    const dim3 grid(blocks_x, n, groups);
+    if (width <= 8) q6k_launch(reorder_pages_kernel<V, 8>, grid, RE_THREADS, 0, st, t, table, blocks, page_size, parents, first, lengths, width);
+    else q6k_launch(reorder_pages_kernel<V, RE_MAX_WIDTH>, grid, RE_THREADS, 0, st, t, table, blocks, page_size, parents, first, lengths, width);
+}
+
+template <typename V>
+void launch_slots(const SlotTensors& t, int n, int groups, int width, int blocks_x, const int* slots, const int* parents, cudaStream_t st) {
+    const dim3 grid(blocks_x, n, groups);
+    if (width <= 8) q6k_launch(reorder_slots_kernel<V, 8>, grid, RE_THREADS, 0, st, t, slots, parents, width);
+    else q6k_launch(reorder_slots_kernel<V, RE_MAX_WIDTH>, grid, RE_THREADS, 0, st, t, slots, parents, width);
+}
+
+}  // namespace
+
+Q6K_API int q6k_reorder_max_width() { return RE_MAX_WIDTH; }
+Q6K_API int q6k_reorder_max_tensors() { return RE_TENSORS; }
+
+// bases, heads, pages, row_bytes: n tensors [heads, pages, page_size, row_bytes] on the host's side; table: int32 [groups * width, blocks];
+// parents: int32 [groups, width]; first, lengths: int32 [groups * width].  Row r takes over positions first[r] .. lengths[parent] - 1.
+Q6K_API int q6k_reorder_pages(int n, const long long* bases, const int* heads, const int* pages, const int* row_bytes, const int* table, int groups, int width,
+                              int blocks, int page_size, const int* parents, const int* first, const int* lengths, cudaStream_t st) {
+    if (n == 0 || groups == 0 || blocks == 0) return 0;
+    Q6K_REQUIRE(n > 0 && n <= RE_TENSORS && groups > 0 && groups <= 65535 && width >= 1 && width <= RE_MAX_WIDTH && blocks > 0 && page_size > 0,
+                "reorder_pages: %d tensors (at most %d), %d groups of %d rows (at most %d), %d blocks of %d", n, RE_TENSORS, groups, width, RE_MAX_WIDTH, blocks, page_size);
+    PageTensors t;
+    unsigned long long all = 0;
+    long long most = 0;
+    for (int i = 0; i < n; ++i) {
+        Q6K_REQUIRE(heads[i] > 0 && pages[i] > 0 && row_bytes[i] > 0, "reorder_pages: tensor %d has %d heads, %d pages, rows of %d bytes", i, heads[i], pages[i], row_bytes[i]);
+        t.base[i] = (char*)bases[i], t.heads[i] = heads[i], t.pages[i] = pages[i], t.row_bytes[i] = row_bytes[i];
+        all |= (unsigned long long)bases[i] | (unsigned long long)row_bytes[i];
+        const long long bytes = (long long)heads[i] * row_bytes[i];
+        if (bytes > most) most = bytes;
+    }
+    const int vb = vector_bytes(all);
+    // enough blocks for every position of the table, at most eight rounds of the GPU's
+    const long long places = (long long)blocks * page_size * (most / vb), want = (places + RE_THREADS - 1) / RE_THREADS, cap = (148 * 8 * 8 + (long long)n * groups - 1) / ((long long)n * groups);
+    const int bx = (int)(want < cap ? want : cap);
+    if (vb == 16) launch_pages<uint4>(t, n, groups, width, bx, table, blocks, page_size, parents, first, lengths, st);
+    else if (vb == 4) launch_pages<uint32_t>(t, n, groups, width, bx, table, blocks, page_size, parents, first, lengths, st);
+    else launch_pages<uint8_t>(t, n, groups, width, bx, table, blocks, page_size, parents, first, lengths, st);
+    return q6k_check_launch("reorder_pages");
+}
+
+// bases, slots, bytes: n tensors [slots, bytes]; slot_ids: int32 [groups * width]; parents: int32 [groups, width].
+Q6K_API int q6k_reorder_slots(int n, const long long* bases, const int* slots, const long long* bytes, const int* slot_ids, int groups, int width, const int* parents,
+                              cudaStream_t st) {
+    if (n == 0 || groups == 0) return 0;
+    Q6K_REQUIRE(n > 0 && n <= RE_TENSORS && groups > 0 && groups <= 65535 && width >= 1 && width <= RE_MAX_WIDTH,
+                "reorder_slots: %d tensors (at most %d), %d groups of %d rows (at most %d)", n, RE_TENSORS, groups, width, RE_MAX_WIDTH);
+    SlotTensors t;
+    unsigned long long all = 0;
+    long long most = 0;
+    for (int i = 0; i < n; ++i) {
+        Q6K_REQUIRE(slots[i] > 0 && bytes[i] > 0, "reorder_slots: tensor %d has %d slots of %lld bytes", i, slots[i], bytes[i]);
+        t.base[i] = (char*)bases[i], t.slots[i] = slots[i], t.bytes[i] = bytes[i];
+        all |= (unsigned long long)bases[i] | (unsigned long long)bytes[i];
+        if (bytes[i] > most) most = bytes[i];
+    }
+    const int vb = vector_bytes(all);
+    const long long want = (most / vb + RE_THREADS - 1) / RE_THREADS, cap = (148 * 8 * 8 + (long long)n * groups - 1) / ((long long)n * groups);
+    const int bx = (int)(want < cap ? want : cap);
+    if (vb == 16) launch_slots<uint4>(t, n, groups, width, bx, slot_ids, parents, st);
+    else if (vb == 4) launch_slots<uint32_t>(t, n, groups, width, bx, slot_ids, parents, st);
+    else launch_slots<uint8_t>(t, n, groups, width, bx, slot_ids, parents, st);
+    return q6k_check_launch("reorder_slots");
+}

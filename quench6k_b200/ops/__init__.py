@@ -2033,3 +2033,239 @@ def hyper_step(x: torch.Tensor, S: int, add=None, read=None, rows: Optional[torc
           _ptr(py), _ptr(pair_row), _ptr(pw), _i(K), _ptr(b), _i(nb), _ptr(wa), _ptr(wb), _f(mult), _ptr(mix), _ptr(out_w), _ptr(in_w), _ptr(norm_w), _f(eps),
           _ptr(out), _ptr(rows), _i(R), _i(S), _i(D), _i(dtype_code(out_dtype)), _stream())
     return dst, out
+
+
+# --------------------------------------------------------------------------- products in 8-bit integers
+def _need_here(t: torch.Tensor, name: str):
+    """The kernels run on the current device's stream: an operand on another device would be read there."""
+    if not t.is_cuda:
+        raise KernelError(f"{name} is on {t.device}; the kernels run on a CUDA device only")
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _need_rows(t: torch.Tensor, name: str):
+    """A matrix whose rows may lie apart."""
+    _need_here(t, name)
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise KernelError(f"{name} has shape {tuple(t.shape)} and strides {tuple(t.stride())}, expected rows of neighbouring values")
+
+
+def quantize_rows(x: torch.Tensor):
+    """(q int8 [R, K], scale float32 [R]) of x [R, K] (float32 or bfloat16; its rows may lie apart): with a the largest |x| of a
+    row and u = 127 / a, q = rint(x u) (ties to even) and scale = a / 127, each rounded to float32 once; an entry stands for
+    q * scale.  A row of zeros (or of values below 3.8e-37, where u is infinite) has the scale 0; a row with a value that is
+    not finite has zeros and the scale NaN."""
+    code = dtype_code(x.dtype)
+    _need_rows(x, "x")
+    R, K = x.shape
+    if K < 1:
+        raise KernelError("quantize_rows: rows without values")
+    q = torch.empty((R, K), dtype=torch.int8, device=x.device)
+    scale = torch.empty(R, dtype=torch.float32, device=x.device)
+    _call("q6k_quantize_rows", _ptr(x), _ll(x.stride(0) if R > 1 else K), _i(R), _i(K), _i(code), _ptr(q), _ptr(scale), _stream())
+    return q, scale
+
+
+def _i8_weights(w, w_scale, w2, w2_scale, K: int, grouped: bool, who: str):
+    """The checks that gemm_i8 and linear_i8 share; (matrices, N)."""
+    _need_here(w, "w")
+    _need(w, "w", torch.int8)
+    if w.dim() != (3 if grouped else 2) or w.shape[-1] != K:
+        raise KernelError(f"{who}: rows of {K} against w of shape {tuple(w.shape)} (three dimensions go with offsets or pair_expert)")
+    if K % 16 or not 0 < K < 131072 or w.data_ptr() % 16:
+        raise KernelError(f"{who}: K={K} must be a multiple of 16 below 131072 and w start on 16 bytes")
+    _need(w_scale, "w_scale", torch.float32, w.shape[:-1])
+    if (w2 is None) != (w2_scale is None):
+        raise KernelError(f"{who}: the second matrix and its scales go together")
+    if w2 is not None:
+        _need(w2, "w2", torch.int8, w.shape)
+        _need(w2_scale, "w2_scale", torch.float32, w.shape[:-1])
+        if w2.data_ptr() % 16:
+            raise KernelError(f"{who}: w2 must start on 16 bytes")
+    return (w.shape[0] if grouped else 1), w.shape[-2]
+
+
+def _i8_out(out, rows: int, N: int, epi: int, device, who: str):
+    dtype = torch.float32 if (epi & 255) in (EPI_STORE, EPI_ADD) else torch.bfloat16
+    if out is None:
+        if (epi & 255) == EPI_ADD:
+            raise KernelError(f"{who}: accumulate needs an output")
+        return torch.empty((rows, N), dtype=dtype, device=device)
+    _need(out, "out", dtype)
+    if out.dim() != 2 or out.shape[0] < rows or out.shape[1] != N:
+        raise KernelError(f"{who}: out has shape {tuple(out.shape)}, needs [{rows}, {N}]")
+    return out
+
+
+def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
+            accumulate: bool = False, w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None,
+            offsets: Optional[torch.Tensor] = None, a_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[r, n] = a_scale[r] * w_scale[n] * sum_k a[r, k] w[n, k] of int8 operands, the sum exact in 32-bit integers.
+
+    a: int8 [*, K], a_scale: float32 [*]; w: int8 [N, K] with w_scale float32 [N].  Stored in float32, or added into `out`
+    (accumulate).  With w2 the gated epilogue act(y) * y2 (act None: silu), with act alone act(y); both leave in bfloat16.
+    a_rows (int32 [rows]): row r of the product is row a_rows[r] of a.  offsets (int32 [G + 1], ascending from 0) with w [G, N, K]
+    and w_scale [G, N]: rows offsets[g] .. offsets[g + 1] - 1 go against matrix g; rows behind the last offset are left as they were."""
+    _need_rows(a, "a")
+    if a.dtype != torch.int8:
+        raise KernelError(f"a has dtype {a.dtype}, expected torch.int8")
+    total, K = a.shape
+    _need(a_scale, "a_scale", torch.float32, (total,))
+    if a.data_ptr() % 16 or (total > 1 and a.stride(0) % 16):
+        raise KernelError("gemm_i8: the rows of a must start on 16 bytes")
+    grouped = offsets is not None
+    groups, N = _i8_weights(w, w_scale, w2, w2_scale, K, grouped, "gemm_i8")
+    epi = _epilogue(w2, accumulate, act)
+    if accumulate and w2 is not None:
+        raise KernelError("gemm_i8: a gated product is stored, not added")
+    if grouped:
+        _need(offsets, "offsets", torch.int32, (groups + 1,))
+    if a_rows is not None:
+        _need(a_rows, "a_rows", torch.int32)
+    rows = a_rows.numel() if a_rows is not None else total
+    out = _i8_out(out, rows, N, epi, a.device, "gemm_i8")
+    _call("q6k_gemm_i8_rows", _ptr(a), _ll(a.stride(0) if total > 1 else K), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
+          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _stream())
+    return out
+
+
+def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool = False,
+              w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None, pair_expert: Optional[torch.Tensor] = None,
+              pair_div: int = 1) -> torch.Tensor:
+    """The product of quantize_rows(x) with weights in 8 bits: x float32 or bfloat16 [T, K], the rest as in gemm_i8.  With
+    pair_expert (int32 [pairs]) and w [experts, N, K]: row y of the result is row y // pair_div of x against the matrix of expert
+    pair_expert[y]; a pair that names no matrix is left as it was."""
+    q, scale = quantize_rows(x)
+    if pair_expert is None:
+        return gemm_i8(q, scale, w, w_scale, out=out, accumulate=accumulate, w2=w2, w2_scale=w2_scale, act=act)
+    T, K = x.shape
+    groups, N = _i8_weights(w, w_scale, w2, w2_scale, K, True, "linear_i8")
+    _need(pair_expert, "pair_expert", torch.int32)
+    pairs = pair_expert.numel()
+    if pair_div < 1 or -(-pairs // pair_div) > T or pairs > 65535:
+        raise KernelError(f"linear_i8: {pairs} pairs (at most 65535), {pair_div} for each of {T} rows")
+    epi = _epilogue(w2, accumulate, act)
+    if accumulate and w2 is not None:
+        raise KernelError("linear_i8: a gated product is stored, not added")
+    out = _i8_out(out, pairs, N, epi, x.device, "linear_i8")
+    _call("q6k_gemm_i8_rows", _ptr(q), _ll(K), _ptr(scale), _i(pairs), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
+          _ptr(None), _ptr(None), _i(groups), _ptr(pair_expert), _i(pair_div), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _stream())
+    return out
+
+
+# --------------------------------------------------------------------------- beam search
+BEAM_MAX_WIDTH, BEAM_MAX_COUNT = 32, 256
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int):
+    """(scores float32, beams int32, tokens int32), each [requests, count]: for every request the `count` best continuations of its
+    beams, t[b, v] = scores[b] + logits[b, v] - log sum_v exp logits[b, v], in descending order, the lowest beam and token first
+    among equals.  logits: float32 [requests * width, V], a request's beams in neighbouring rows; scores: float32 [requests, width].
+    A continuation whose beam's score, logit or row sum is not finite counts as -infinity and comes after all others (a beam
+    of score -infinity takes no part while others have continuations left).  t is compared in 64 bits and rounded on the way out."""
+    _need_here(logits, "logits")
+    _need(logits, "logits", torch.float32)
+    _need(scores, "scores", torch.float32)
+    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
+        raise KernelError(f"beam_select: logits {tuple(logits.shape)} for scores {tuple(scores.shape)}")
+    requests, width = scores.shape
+    V = logits.shape[1]
+    count = int(count)
+    if not 1 <= width <= BEAM_MAX_WIDTH or not 1 <= count <= min(BEAM_MAX_COUNT, width * V) or width * V >= 1 << 31 or requests * width > 65535:
+        raise KernelError(f"beam_select: {count} continuations (1 to {BEAM_MAX_COUNT}) of {requests} requests of {width} beams (1 to {BEAM_MAX_WIDTH}) over {V} tokens")
+    lib = library()
+    lib.q6k_beam_scratch.restype = ctypes.c_longlong
+    nbytes = lib.q6k_beam_scratch(_i(requests * width), _i(V), _i(count))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    out = torch.empty((requests, count), dtype=torch.float32, device=logits.device)
+    where = torch.empty((2, requests, count), dtype=torch.int32, device=logits.device)
+    beams, tokens = where.unbind(0)
+    _call("q6k_beam_select", _ptr(logits), _ptr(scores), _i(requests), _i(width), _i(V), _i(count), _ptr(scratch), _ll(nbytes), _ptr(out), _ptr(beams), _ptr(tokens),
+          _stream(), launches=2 if requests else 0)
+    return out, beams, tokens
+
+
+class PageSet:
+    """Paged tensors [heads, pages, page_size, width] that share one block table (the keys and values of a cache group's layers), as
+    reorder_pages takes them; made once and kept beside the tensors."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise KernelError("PageSet: no tensors")
+        self.page_size, self.device = self.tensors[0].shape[2] if self.tensors[0].dim() == 4 else 0, self.tensors[0].device
+        for t in self.tensors:
+            _need(t, "pages")
+            if t.dim() != 4 or t.shape[2] != self.page_size or t.numel() == 0 or t.device != self.device:
+                raise KernelError(f"PageSet: pages of shape {tuple(t.shape)} on {t.device}, expected [heads, pages, {self.page_size}, width] on {self.device}")
+        n = len(self.tensors)
+        ints = lambda values: (ctypes.c_int * n)(*values)
+        self.args = ((ctypes.c_longlong * n)(*[t.data_ptr() for t in self.tensors]), ints([t.shape[0] for t in self.tensors]),
+                     ints([t.shape[1] for t in self.tensors]), ints([t.shape[3] * t.element_size() for t in self.tensors]))
+
+
+class SlotSet:
+    """Tensors [slots, ...] of fixed-size states that share their slot numbers, as reorder_slots takes them; made once and kept."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise KernelError("SlotSet: no tensors")
+        self.device = self.tensors[0].device
+        for t in self.tensors:
+            _need(t, "states")
+            if t.dim() < 1 or t.numel() == 0 or t.device != self.device:
+                raise KernelError(f"SlotSet: states of shape {tuple(t.shape)} on {t.device}, expected [slots, ...] on {self.device}")
+        n = len(self.tensors)
+        self.args = ((ctypes.c_longlong * n)(*[t.data_ptr() for t in self.tensors]), (ctypes.c_int * n)(*[t.shape[0] for t in self.tensors]),
+                     (ctypes.c_longlong * n)(*[t.numel() // t.shape[0] * t.element_size() for t in self.tensors]))
+
+
+def _parents(parents: torch.Tensor, who: str):
+    _need_here(parents, "parents")
+    _need(parents, "parents", torch.int32)
+    if parents.dim() != 2 or not 1 <= parents.shape[1] <= BEAM_MAX_WIDTH or parents.shape[0] > 65535:
+        raise KernelError(f"{who}: parents have shape {tuple(parents.shape)}, expected [groups, 1 to {BEAM_MAX_WIDTH}]")
+    return parents.shape
+
+
+def _batches(args, most: int = 128):
+    """The arguments of a set, at most `most` tensors at a time: what one launch takes."""
+    n = len(args[0])
+    for at in range(0, n, most):
+        m = min(most, n - at)
+        yield (m, *args) if m == n else (m, *[(a._type_ * m)(*a[at:at + m]) for a in args])
+
+
+def reorder_pages(pages, table: torch.Tensor, parents: torch.Tensor, first: torch.Tensor, lengths: torch.Tensor) -> None:
+    """Rows of a group that go on from one another, all at once: row r takes over its parent's positions first[r] ..
+    lengths[parent] - 1 in every tensor of `pages` (a PageSet, or the tensors).  table: int32 [rows, blocks], the page of every
+    logical block, -1 where none is held (what a row does not hold stays as it is); parents: int32 [groups, width], a number
+    within the group for each of its neighbouring rows (its own, or one outside the group: the row stays); first, lengths: int32
+    [rows].  Pages that are written belong to one row only."""
+    if not isinstance(pages, PageSet):
+        pages = PageSet(pages)
+    groups, width = _parents(parents, "reorder_pages")
+    rows = groups * width
+    _need(table, "table", torch.int32)
+    _need(first, "first", torch.int32, (rows,))
+    _need(lengths, "lengths", torch.int32, (rows,))
+    if table.dim() != 2 or table.shape[0] != rows or pages.device != parents.device:
+        raise KernelError(f"reorder_pages: a table of shape {tuple(table.shape)} for {groups} groups of {width} rows on {pages.device}")
+    for n, bases, heads, count, row_bytes in _batches(pages.args):
+        _call("q6k_reorder_pages", _i(n), bases, heads, count, row_bytes, _ptr(table), _i(groups), _i(width), _i(table.shape[1]), _i(pages.page_size), _ptr(parents),
+              _ptr(first), _ptr(lengths), _stream())
+
+
+def reorder_slots(states, slots: torch.Tensor, parents: torch.Tensor) -> None:
+    """The same for fixed-size states: row r's slot slots[r] takes over the slot of its parent, in every tensor of `states` (a
+    SlotSet, or the tensors [slots, ...]).  slots: int32 [rows], no slot twice; a number outside the tensor: nothing is held."""
+    if not isinstance(states, SlotSet):
+        states = SlotSet(states)
+    groups, width = _parents(parents, "reorder_slots")
+    _need(slots, "slots", torch.int32, (groups * width,))
+    if states.device != parents.device:
+        raise KernelError(f"reorder_slots: states on {states.device}, parents on {parents.device}")
+    for n, bases, count, nbytes in _batches(states.args):
+        _call("q6k_reorder_slots", _i(n), bases, count, nbytes, _ptr(slots), _i(groups), _i(width), _ptr(parents), _stream())
