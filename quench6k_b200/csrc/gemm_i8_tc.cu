@@ -1,0 +1,416 @@
+// Products in 8-bit integers on the 5th-generation tensor cores (tcgen05.mma kind::i8, 32-bit integer accumulators in tensor
+// memory), operands brought into shared memory by TMA.  sm_100a only.
+//
+//   y[r, n] = a_scale[r] * w_scale[g, n] * sum_k a[r, k] w[g, n, k]          int8 operands, K contiguous
+//
+// As in the bfloat16 products (gemm_tc.cu) the weights are the M side of the MMA and the rows the N side: a tile of 128 weight
+// rows per CTA against BT rows of a.  A persistent unit (one CTA, or a pair of CTAs that work on one tile of 256 weight rows
+// with cta_group::2) walks the tiles:
+//   warp 0     producer: TMA loads of [128 weights x 128 bytes of k] and [rows x 128 bytes] into a ring of stages
+//   warp 1     tensor memory (two accumulators) and the MMAs, four of K = 32 per stage
+//   others     epilogue: accumulators to registers, the two scales, the store
+// A gated product's tile holds 64 rows of the gate's matrix (lanes 0-63) and the same 64 of the other one (lanes 64-127); the
+// two warps that hold a column's two products exchange half of theirs through shared memory.
+// Grouped products find their tiles from the groups' offsets in the kernel: no tile list is made.
+// Every wait on an mbarrier is bounded; a wait that runs out records a code that q6k_gemm_i8_status() returns, and the roles fall
+// through to the common exit.
+#include "common.cuh"
+#include "gemm_i8.cuh"
+#include "tma.cuh"
+#include "umma.cuh"
+
+namespace {
+
+constexpr int BK = 128;                // int8 per k-block: one 128-byte swizzle row
+constexpr int WM = 128;                // weight rows of a CTA
+constexpr int MAX_STAGES = 10, MAX_GROUPS = 4096;
+constexpr int SWAP_BYTES = 2 * 16 * 32 * 4;      // a gated epilogue warp's 16 rows for its partner, two buffers
+
+__device__ int g_i8_status = 0;
+
+struct TcArgs {
+    I8Args p;
+    int stages, n_x, n_y;              // tiles along N, and along the rows (dense)
+    int w_once;                        // every weight tile is fetched once, or by few units side by side
+};
+
+// D: 32-bit integers, A and B signed 8-bit integers, both K-major, M rows, N = n.
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+template <int CTAS>
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+constexpr uint32_t PEER_MASK = 0xFEFFFFFFu;    // a shared-memory address of either CTA of a pair -> the same offset in the even one
+
+template <int CTAS>
+__device__ __forceinline__ void commit(uint32_t bar) {          // with a pair: at this offset in both CTAs
+    if constexpr (CTAS == 1) umma_commit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                     : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, bool once, uint64_t policy) {
+    if constexpr (CTAS == 1) {
+        if (once) tma_load_2d_once(dst, map, x, y, bar, policy);
+        else tma_load_2d(dst, map, x, y, bar);
+    } else {
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+                     "r"(x), "r"(y), "r"(bar & PEER_MASK)
+                     : "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+    if constexpr (CTAS == 1) mbar_arrive(bar);
+    else asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar & PEER_MASK) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Which weights, which rows.
+struct Tile {
+    int g, n0, row0, row_end;
+};
+
+// Tile t: tiles along N fastest (units side by side share the rows).  starts (grouped): how many row tiles come before each group.
+template <int BT>
+__device__ __forceinline__ Tile tile_of(const TcArgs& a, int t, int cols, const int* starts) {
+    Tile o;
+    const int y = t / a.n_x;
+    o.n0 = t % a.n_x * cols;
+    if (a.p.offsets) {
+        int lo = 0, hi = a.p.groups - 1;                 // the last group with starts[g] <= y (empty groups share their start with the next)
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (starts[mid] <= y) lo = mid;
+            else hi = mid - 1;
+        }
+        o.g = lo;
+        o.row0 = a.p.offsets[lo] + (y - starts[lo]) * BT, o.row_end = min(a.p.offsets[lo + 1], a.p.rows);
+    } else {
+        o.g = 0, o.row0 = y * BT, o.row_end = a.p.rows;
+    }
+    return o;
+}
+
+__device__ __forceinline__ void tmem_ld16_ints(uint32_t taddr, int* v) {
+    float f[16];
+    tmem_ld16_issue(taddr, f);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_int(f[i]);
+}
+
+__host__ __device__ constexpr int epilogue_warps(int bt) { return bt >= 64 ? 8 : 4; }
+
+template <int BT, int CTAS, bool DUAL>
+__global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
+                                                                                    const __grid_constant__ CUtensorMap tm_a, const TcArgs a) {
+    pdl_enter();
+    constexpr int EW = epilogue_warps(BT), SPAN = BT / (EW / 4);       // rows that an epilogue warp takes of a tile
+    constexpr uint32_t W_BYTES = WM * BK, A_BYTES = BT / CTAS * BK, STAGE_BYTES = W_BYTES + A_BYTES;
+    constexpr int COLS = DUAL ? WM / 2 : WM;                           // output columns of a CTA's tile
+    constexpr uint32_t TMEM_COLS = 2 * BT <= 32 ? 32 : 2 * BT <= 64 ? 64 : 2 * BT <= 128 ? 128 : 2 * BT <= 256 ? 256 : 512;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 4];
+    __shared__ uint32_t tmem_slot;
+    const I8Args& p = a.p;
+    const int stages = a.stages, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = smem_u32(smem), swap0 = ring + stages * STAGE_BYTES;
+    int* starts = (int*)(smem + (size_t)stages * STAGE_BYTES + (DUAL ? EW * SWAP_BYTES : 0));
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[MAX_STAGES]);
+    const uint32_t acc_full0 = smem_u32(&bars[2 * MAX_STAGES]), acc_empty0 = smem_u32(&bars[2 * MAX_STAGES + 2]);
+    const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
+    const int unit = blockIdx.x / CTAS, units = gridDim.x / CTAS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
+        for (int b = 0; b < 2; ++b) mbar_init(acc_full0 + 8 * b, 1), mbar_init(acc_empty0 + 8 * b, EW * CTAS);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_a) : "memory");
+    }
+    if (warp == 1) {
+        if constexpr (CTAS == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    } else if (warp == 2 && p.offsets) {                 // row tiles before each group
+        int before = 0;
+        for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            const int rows = g < p.groups ? min(p.offsets[g + 1], p.rows) - p.offsets[g] : 0;
+            const int mine = rows > 0 ? (rows + BT - 1) / BT : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            if (g <= p.groups) starts[g] = before + upto - mine;
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();             // both CTAs' barriers exist before either signals the other
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int total = a.n_x * (p.offsets ? starts[p.groups] : a.n_y), kbs = (p.K + BK - 1) / BK;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            const uint64_t once = l2_evict_first_policy();
+            int s = 0;
+            uint32_t st = ring, phase = 0;
+            bool ok = true;
+            for (int t = unit; t < total && ok; t += units) {
+                const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
+                const int wy = tl.g * p.N + tl.n0 + rank * COLS, ay = tl.row0 + rank * (BT / CTAS);
+                for (int i = 0; i < kbs; ++i) {
+                    const uint32_t fb = full0 + 8 * s;
+                    if (!mbar_wait(empty0 + 8 * s, phase ^ 1)) {
+                        atomicExch(&g_i8_status, 21);
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_expect_tx(fb, CTAS * STAGE_BYTES);
+                    load<CTAS>(st, &tm_w, i * BK, wy, fb, a.w_once, once);
+                    if (DUAL) load<CTAS>(st + W_BYTES / 2, &tm_w2, i * BK, wy, fb, a.w_once, once);
+                    load<CTAS>(st + W_BYTES, &tm_a, i * BK, ay, fb, false, once);
+                    if (++s == stages) s = 0, st = ring, phase ^= 1;
+                    else st += STAGE_BYTES;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            constexpr uint32_t idesc = idesc_i8(CTAS * WM, BT);
+            int s = 0, nt = 0;
+            uint32_t st = ring, phase = 0;
+            bool ok = true;
+            for (int t = unit; t < total && ok; t += units, ++nt) {
+                const int buf = nt & 1;
+                if (!mbar_wait(acc_empty0 + 8 * buf, ((nt >> 1) & 1) ^ 1)) {
+                    atomicExch(&g_i8_status, 24);
+                    break;
+                }
+                tc_fence_after();
+                for (int i = 0; i < kbs; ++i) {
+                    if (!mbar_wait(full0 + 8 * s, phase)) {
+                        atomicExch(&g_i8_status, 22);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t dw = umma_desc_k(st), da = umma_desc_k(st + W_BYTES);
+#pragma unroll
+                    for (int k = 0; k < BK / 32; ++k) umma_i8<CTAS>(tmem + buf * BT, dw + 2 * k, da + 2 * k, idesc, (i | k) != 0);      // + 32 bytes of k per step
+                    commit<CTAS>(empty0 + 8 * s);
+                    if (++s == stages) s = 0, st = ring, phase ^= 1;
+                    else st += STAGE_BYTES;
+                }
+                if (ok) commit<CTAS>(acc_full0 + 8 * buf);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, part = (warp - 2) >> 2;           // lanes 32 quarter .. of the accumulator, rows part * SPAN .. of the tile
+        const bool gate = quarter < 2;
+        const uint32_t mine = swap0 + (warp - 2) * SWAP_BYTES, theirs = swap0 + ((part << 2 | ((quarter ^ 2) + 2 & 3)) * SWAP_BYTES);
+        int nt = 0, turn = 0;
+        bool ok = true;
+        for (int t = unit; t < total; t += units, ++nt) {
+            const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
+            const int buf = nt & 1, n = tl.n0 + rank * COLS + (DUAL ? quarter & 1 : quarter) * 32 + lane;
+            const float ws = n < p.N ? ((DUAL && !gate) ? p.w2_scale : p.w_scale)[(long long)tl.g * p.N + n] : 0.0f;
+            const int end = min(SPAN, tl.row_end - tl.row0 - part * SPAN), row0 = tl.row0 + part * SPAN;
+            auto row_scale = [&](int c0) {               // lane j: the scale of row c0 + j
+                const int r = row0 + c0 + (lane & (DUAL ? 31 : 15));
+                return r < tl.row_end ? p.a_scale[p.a_rows ? p.a_rows[r] : r] : 0.0f;
+            };
+            float next = row_scale(0);
+            if (ok && !mbar_wait(acc_full0 + 8 * buf, (nt >> 1) & 1)) {
+                if (lane == 0) atomicExch(&g_i8_status, 23);
+                ok = false;                              // on to the barriers that a partner may be waiting at, with no further wait
+            }
+            tc_fence_after();
+            const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BT + part * SPAN;
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader<CTAS>(acc_empty0 + 8 * buf);
+            };
+            if (end <= 0) release();
+            if constexpr (DUAL) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < end; c0 += 32, ++turn) {
+                    int v[16], u[16];
+                    tmem_ld16_ints(from + c0 + (gate ? 0 : 16), v);
+                    tmem_ld16_ints(from + c0 + (gate ? 16 : 0), u);
+                    if (c0 + 32 >= end) release();
+                    const float xs = next;
+                    next = row_scale(c0 + 32);
+                    const uint32_t at = (turn & 1) * (SWAP_BYTES / 2) + lane * 4;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float f = (float)u[j] * (__shfl_sync(0xffffffffu, xs, j + (gate ? 16 : 0)) * ws);
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + at + j * 128), "f"(f) : "memory");
+                    }
+                    // both have written; and the buffers of the turn before have been read
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + part * 2 + (quarter & 1)) : "memory");
+                    const int first = c0 + (gate ? 0 : 16);
+                    __nv_bfloat16* o = (__nv_bfloat16*)p.out + (long long)(row0 + first) * p.ldo + n;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float other;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(theirs + at + j * 128) : "memory");
+                        const float f = (float)v[j] * (__shfl_sync(0xffffffffu, xs, j + (gate ? 0 : 16)) * ws);
+                        const float y = q6k_gated(gate ? f : other, gate ? other : f, p.act, p.act_param);
+                        if (n < p.N && first + j < end) o[(long long)j * p.ldo] = __float2bfloat16_rn(y);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int c0 = 0; c0 < end; c0 += 16) {
+                    int v[16];
+                    tmem_ld16_ints(from + c0, v);
+                    if (c0 + 16 >= end) release();
+                    const float xs = next;
+                    next = row_scale(c0 + 16);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float f = (float)v[j] * (__shfl_sync(0xffffffffu, xs, j) * ws);
+                        if (n < p.N && c0 + j < end) {
+                            const long long at = (long long)(row0 + c0 + j) * p.ldo + n;
+                            if (p.epilogue == I8_ADD) atomicAdd((float*)p.out + at, f);      // nobody else adds here: one addition, without waiting for what is there
+                            else if (p.epilogue == I8_ACT) ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(q6k_activation(f, p.act));
+                            else ((float*)p.out)[at] = f;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();             // the peer has no MMA, copy or arrival of ours in flight
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------------- host
+// An int8 matrix [rows, cols] in boxes of [box_rows, 128] with the 128-byte swizzle; reads outside give zeros.
+int make_i8_map(CUtensorMap* map, const void* base, long long rows, int cols, long long pitch, int box_rows, bool weights) {
+    EncodeTiled fn = encode_fn();
+    if (!fn) return q6k_fail("gemm_i8: the driver does not offer cuTensorMapEncodeTiled");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, weights ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return q6k_fail("gemm_i8: cuTensorMapEncodeTiled failed with code %d (%lld rows of %d, pitch %lld, box %d)", (int)r, rows, cols, pitch, box_rows);
+    return 0;
+}
+
+int sm_count() {
+    static int n = 0;
+    if (!n) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    }
+    return n;
+}
+
+template <int BT, int CTAS, bool DUAL>
+int launch(const TcArgs& args, int a_total, cudaStream_t st) {
+    TcArgs t = args;
+    const I8Args& p = t.p;
+    constexpr int EW = epilogue_warps(BT), COLS = CTAS * (DUAL ? WM / 2 : WM);
+    constexpr int stage = WM * BK + BT / CTAS * BK;
+    CUtensorMap tw, tw2, ta;
+    const int w_box = DUAL ? WM / 2 : WM;
+    if (int rc = make_i8_map(&tw, p.w, (long long)p.groups * p.N, p.K, p.K, w_box, true)) return rc;
+    tw2 = tw;
+    if (DUAL)
+        if (int rc = make_i8_map(&tw2, p.w2, (long long)p.groups * p.N, p.K, p.K, w_box, true)) return rc;
+    if (int rc = make_i8_map(&ta, p.a, a_total, p.K, p.lda, BT / CTAS, false)) return rc;
+    const int extra = (DUAL ? EW * SWAP_BYTES : 0) + (p.offsets ? (p.groups + 1) * 4 : 0);
+    t.stages = (222 * 1024 - extra) / stage;
+    if (t.stages > MAX_STAGES) t.stages = MAX_STAGES;
+    t.n_x = (p.N + COLS - 1) / COLS, t.n_y = (p.rows + BT - 1) / BT;
+    const long long row_tiles = p.offsets ? p.rows / BT + (p.groups < p.rows ? p.groups : p.rows) : t.n_y, total = t.n_x * row_tiles;
+    Q6K_REQUIRE(total < (1LL << 31), "gemm_i8: %lld tiles", total);
+    t.w_once = p.offsets ? p.rows <= 2LL * p.groups * BT : t.n_y == 1;
+    const size_t smem = (size_t)t.stages * stage + extra + 1024;
+    static bool configured = false;
+    if (!configured) {
+        if (cudaFuncSetAttribute(gemm_i8_tc_kernel<BT, CTAS, DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess)
+            return q6k_check_launch("gemm_i8: shared memory attribute");
+        configured = true;
+    }
+    const int units = sm_count() / CTAS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(CTAS * (unsigned)(total < units ? total : units)), cfg.blockDim = dim3(64 + 32 * EW), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = CTAS == 2 ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, gemm_i8_tc_kernel<BT, CTAS, DUAL>, tw, tw2, ta, t);
+    return q6k_check_launch("gemm_i8");
+}
+
+}  // namespace
+
+Q6K_API int q6k_gemm_i8_status() {
+    int v = -1;
+    if (cudaMemcpyFromSymbol(&v, g_i8_status, sizeof v) != cudaSuccess) return -1;
+    return v;
+}
+
+// See ops.gemm_i8 for the operands.  a_rows: the rows of a have been gathered already, the list is for their scales; a has `a_total` rows.
+// tile: rows of a tile (0: chosen here), negative for pairs of CTAs.
+Q6K_API int q6k_gemm_i8_tc(I8_OPERANDS, int a_total, int tile, cudaStream_t st) {
+    TcArgs t;
+    if (int rc = i8_args(&t.p, "gemm_i8", I8_NAMES)) return rc;
+    if (rows == 0) return 0;
+    Q6K_REQUIRE(!pair_expert && groups <= MAX_GROUPS && (long long)groups * N < (1LL << 31) - 256 && a_total >= rows, "gemm_i8: %d groups of %d columns, %d rows of %d", groups, N, rows, a_total);
+    const bool dual = w2 != nullptr;
+    if (tile == 0) tile = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+#define GO(T_, BT_, CTAS_) \
+    case T_: return dual ? launch<BT_, CTAS_, true>(t, a_total, st) : launch<BT_, CTAS_, false>(t, a_total, st)
+    switch (tile) {
+        GO(32, 32, 1);
+        GO(64, 64, 1);
+        GO(128, 128, 1);
+        GO(256, 256, 1);
+        GO(-192, 192, 2);
+        GO(-256, 256, 2);
+    }
+#undef GO
+    return q6k_fail("gemm_i8: tiles of %d rows", tile);
+}

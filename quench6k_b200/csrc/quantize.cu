@@ -1,7 +1,8 @@
-// Rows in 8 bits: with a = max |x[r, :]|, u = 127 / a (rounded to FP32) the entries are q = rint(x u), whole numbers from -127 to
-// 127 (ties to even), and an entry stands for q * scale with scale = a / 127.
+// Rows in 8 bits: with a = max |x[r, :]| and u = (1 / a) * 127 the entries are q = rint(x u), whole numbers from -127 to 127 (ties
+// to even), and an entry stands for q * scale with scale = a * (1 / 127).  Each quotient and product is rounded to FP32 once, so
+// that q and scale are the same wherever they are computed.
 //
-// A row of zeros, or one so small that 127 / a is infinite (a < 3.8e-37), gets zeros and the scale 0; a row with a value that
+// A row of zeros, or one so small that u is infinite (a < 3.8e-37), gets zeros and the scale 0; a row with a value that
 // is not finite gets zeros and the scale NaN, so that every product with it is NaN.
 #include "common.cuh"
 
@@ -25,9 +26,9 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long lon
     for (int w = 0; w < 8; ++w) most = max(most, most_of_warp[w]);
     const float a = __uint_as_float(most);
     const bool finite = most < 0x7f800000u;
-    float u = 127.0f / a;
+    const float u = 1.0f / a * 127.0f;
     const bool zero = !finite || abs_bits(u) >= 0x7f800000u;
-    if (threadIdx.x == 0) scale[blockIdx.x] = !finite ? __uint_as_float(0x7fffffffu) : zero ? 0.0f : a / 127.0f;
+    if (threadIdx.x == 0) scale[blockIdx.x] = !finite ? __uint_as_float(0x7fffffffu) : zero ? 0.0f : a * (1.0f / 127.0f);
     for (int k = threadIdx.x; k < K; k += 256) out[k] = zero ? (int8_t)0 : (int8_t)__float2int_rn(to_f32(row[k]) * u);
 }
 

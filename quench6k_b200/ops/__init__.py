@@ -377,7 +377,8 @@ def tc_status() -> int:
     lib.q6k_router_status.restype = ctypes.c_int
     lib.q6k_attention_flex_tc_status.restype = ctypes.c_int
     lib.q6k_retention_tc_status.restype = ctypes.c_int
-    return (lib.q6k_retention_tc_status() or lib.q6k_tc_status() or lib.q6k_attention_status() or lib.q6k_attention_tc_status() or lib.q6k_attention_flex_tc_status()
+    lib.q6k_gemm_i8_status.restype = ctypes.c_int
+    return (lib.q6k_gemm_i8_status() or lib.q6k_retention_tc_status() or lib.q6k_tc_status() or lib.q6k_attention_status() or lib.q6k_attention_tc_status() or lib.q6k_attention_flex_tc_status()
             or lib.q6k_router_status())
 
 
@@ -2053,8 +2054,8 @@ def _need_rows(t: torch.Tensor, name: str):
 
 def quantize_rows(x: torch.Tensor):
     """(q int8 [R, K], scale float32 [R]) of x [R, K] (float32 or bfloat16; its rows may lie apart): with a the largest |x| of a
-    row and u = 127 / a, q = rint(x u) (ties to even) and scale = a / 127, each rounded to float32 once; an entry stands for
-    q * scale.  A row of zeros (or of values below 3.8e-37, where u is infinite) has the scale 0; a row with a value that is
+    row and u = (1 / a) * 127, q = rint(x u) (ties to even) and scale = a * (1 / 127), every step rounded to float32; an entry stands
+    for q * scale.  A row of zeros (or of values below 3.8e-37, where u is infinite) has the scale 0; a row with a value that is
     not finite has zeros and the scale NaN."""
     code = dtype_code(x.dtype)
     _need_rows(x, "x")
@@ -2098,6 +2099,9 @@ def _i8_out(out, rows: int, N: int, epi: int, device, who: str):
     return out
 
 
+_i8_tile = 0
+
+
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
             accumulate: bool = False, w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None,
             offsets: Optional[torch.Tensor] = None, a_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2125,8 +2129,17 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
         _need(a_rows, "a_rows", torch.int32)
     rows = a_rows.numel() if a_rows is not None else total
     out = _i8_out(out, rows, N, epi, a.device, "gemm_i8")
-    _call("q6k_gemm_i8_rows", _ptr(a), _ll(a.stride(0) if total > 1 else K), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _stream())
+    lda = a.stride(0) if total > 1 else K
+    if rows <= 16 and not grouped:
+        _call("q6k_gemm_i8_rows", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
+              _ptr(a_rows), _ptr(None), _i(1), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _stream())
+        return out
+    if a_rows is not None:
+        if not a.is_contiguous():
+            raise KernelError("gemm_i8: rows that are picked lie side by side")
+        a, total, lda = gather_rows(a, a_rows), rows, K
+    _call("q6k_gemm_i8_tc", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
+          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(total), _i(_i8_tile), _stream())
     return out
 
 

@@ -14,12 +14,12 @@ def quantized(x):
     x = np.asarray(x, dtype=np.float32)
     a = np.abs(x).max(axis=1)
     with np.errstate(divide="ignore", invalid="ignore", over="ignore"):
-        u = np.float32(127.0) / a
+        u = np.float32(1) / a * np.float32(127)
         finite = np.isfinite(a)
         zero = ~finite | ~np.isfinite(u)
         q = np.rint(x * np.where(zero, np.float32(0), u)[:, None])
     q = np.where(zero[:, None], 0, np.nan_to_num(q)).astype(np.int8)
-    return q, np.where(~finite, np.float32(np.nan), np.where(zero, np.float32(0), a / np.float32(127.0))).astype(np.float32)
+    return q, np.where(~finite, np.float32(np.nan), np.where(zero, np.float32(0), a * (np.float32(1) / np.float32(127)))).astype(np.float32)
 
 
 def rows_of(seed, rows, cols, dtype, apart=0):
