@@ -36,10 +36,15 @@ inline int i8_args(I8Args* p, const char* who, I8_OPERANDS) {
     return 0;
 }
 
+// silu(g) u by a fast quotient: it is off by some 2^-21 of the value, and the result is rounded to bfloat16 (2^-8); where e^-g is beyond 2^126 the value
+// is below 1e-36 and comes out as zero.
+__device__ __forceinline__ float i8_silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+__device__ __forceinline__ float i8_gated(float g, float u, int act, float param) { return act == 0 ? i8_silu_times(g, u) : q6k_gated(g, u, act, param); }
+
 // v (and u, the second matrix's) is the scaled product that belongs at out[at].
 template <bool DUAL>
 __device__ __forceinline__ void i8_store(const I8Args& p, long long at, float v, float u) {
-    if (DUAL) ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(q6k_gated(v, u, p.act, p.act_param));
+    if (DUAL) ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(i8_gated(v, u, p.act, p.act_param));
     else if (p.epilogue == I8_ACT) ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(q6k_activation(v, p.act));
     else if (p.epilogue == I8_ADD) ((float*)p.out)[at] += v;
     else ((float*)p.out)[at] = v;

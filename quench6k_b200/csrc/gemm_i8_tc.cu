@@ -25,6 +25,7 @@ constexpr int BK = 128;                // int8 per k-block: one 128-byte swizzle
 constexpr int WM = 128;                // weight rows of a CTA
 constexpr int MAX_STAGES = 10, MAX_GROUPS = 4096;
 constexpr int SWAP_BYTES = 2 * 16 * 32 * 4;      // a gated epilogue warp's 16 rows for its partner, two buffers
+constexpr int SCALE_BYTES = 128 * 4;             // an epilogue warp's rows' scales
 
 __device__ int g_i8_status = 0;
 
@@ -111,14 +112,6 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, int t, int cols, const 
     return o;
 }
 
-__device__ __forceinline__ void tmem_ld16_ints(uint32_t taddr, int* v) {
-    float f[16];
-    tmem_ld16_issue(taddr, f);
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __float_as_int(f[i]);
-}
-
 __host__ __device__ constexpr int epilogue_warps(int bt) { return bt >= 64 ? 8 : 4; }
 
 template <int BT, int CTAS, bool DUAL>
@@ -136,7 +129,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     const I8Args& p = a.p;
     const int stages = a.stages, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ring = smem_u32(smem), swap0 = ring + stages * STAGE_BYTES;
-    int* starts = (int*)(smem + (size_t)stages * STAGE_BYTES + (DUAL ? EW * SWAP_BYTES : 0));
+    const uint32_t scales0 = swap0 + (DUAL ? EW * SWAP_BYTES : 0);
+    int* starts = (int*)(smem + (size_t)stages * STAGE_BYTES + (DUAL ? EW * SWAP_BYTES : 0) + EW * SCALE_BYTES);
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[MAX_STAGES]);
     const uint32_t acc_full0 = smem_u32(&bars[2 * MAX_STAGES]), acc_empty0 = smem_u32(&bars[2 * MAX_STAGES + 2]);
     const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
@@ -244,13 +238,25 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
         for (int t = unit; t < total; t += units, ++nt) {
             const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
             const int buf = nt & 1, n = tl.n0 + rank * COLS + (DUAL ? quarter & 1 : quarter) * 32 + lane;
-            const float ws = n < p.N ? ((DUAL && !gate) ? p.w2_scale : p.w_scale)[(long long)tl.g * p.N + n] : 0.0f;
+            const long long at_n = (long long)tl.g * p.N + n;
+            const float ws = n < p.N ? p.w_scale[at_n] : 0.0f, ws2 = DUAL && n < p.N ? p.w2_scale[at_n] : 0.0f;
             const int end = min(SPAN, tl.row_end - tl.row0 - part * SPAN), row0 = tl.row0 + part * SPAN;
-            auto row_scale = [&](int c0) {               // lane j: the scale of row c0 + j
-                const int r = row0 + c0 + (lane & (DUAL ? 31 : 15));
-                return r < tl.row_end ? p.a_scale[p.a_rows ? p.a_rows[r] : r] : 0.0f;
+            // the rows' scales go to shared memory while the accumulator fills (read from global memory where they are needed, every 16 rows waited for them:
+            // 2,048 x 2,048 x 2,048 16.0 us, 12.1 now)
+            const uint32_t scales = scales0 + (warp - 2) * SCALE_BYTES;
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < SPAN; c += 32) {
+                const int r = row0 + c + lane;
+                const float xs = r < tl.row_end ? p.a_scale[p.a_rows ? p.a_rows[r] : r] : 0.0f;
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + (c + lane) * 4), "f"(xs) : "memory");
+            }
+            __syncwarp();
+            auto scales_of = [&](int c0, float* xs) {    // of 16 rows
+#pragma unroll
+                for (int j = 0; j < 16; j += 4)
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(xs[j]), "=f"(xs[j + 1]), "=f"(xs[j + 2]), "=f"(xs[j + 3]) : "r"(scales + (c0 + j) * 4) : "memory");
             };
-            float next = row_scale(0);
             if (ok && !mbar_wait(acc_full0 + 8 * buf, (nt >> 1) & 1)) {
                 if (lane == 0) atomicExch(&g_i8_status, 23);
                 ok = false;                              // on to the barriers that a partner may be waiting at, with no further wait
@@ -266,48 +272,85 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
             if constexpr (DUAL) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < end; c0 += 32, ++turn) {
-                    int v[16], u[16];
-                    tmem_ld16_ints(from + c0 + (gate ? 0 : 16), v);
-                    tmem_ld16_ints(from + c0 + (gate ? 16 : 0), u);
+                    float v[16], u[16];                  // 32-bit integers until they are scaled
+                    tmem_ld16_issue(from + c0 + (gate ? 0 : 16), v);
+                    tmem_ld16_issue(from + c0 + (gate ? 16 : 0), u);
+                    tmem_ld_wait();
                     if (c0 + 32 >= end) release();
-                    const float xs = next;
-                    next = row_scale(c0 + 32);
                     const uint32_t at = (turn & 1) * (SWAP_BYTES / 2) + lane * 4;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float f = (float)u[j] * (__shfl_sync(0xffffffffu, xs, j + (gate ? 16 : 0)) * ws);
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + at + j * 128), "f"(f) : "memory");
-                    }
+                    for (int j = 0; j < 16; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + at + j * 128), "f"(u[j]) : "memory");
                     // both have written; and the buffers of the turn before have been read
                     asm volatile("bar.sync %0, 64;" ::"r"(1 + part * 2 + (quarter & 1)) : "memory");
-                    const int first = c0 + (gate ? 0 : 16);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(u[j]) : "r"(theirs + at + j * 128) : "memory");
+                    const int first = c0 + (gate ? 0 : 16), rows = n < p.N ? end - first : 0;
+                    float xs[16];
+                    scales_of(first, xs);
                     __nv_bfloat16* o = (__nv_bfloat16*)p.out + (long long)(row0 + first) * p.ldo + n;
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        float other;
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(theirs + at + j * 128) : "memory");
-                        const float f = (float)v[j] * (__shfl_sync(0xffffffffu, xs, j + (gate ? 0 : 16)) * ws);
-                        const float y = q6k_gated(gate ? f : other, gate ? other : f, p.act, p.act_param);
-                        if (n < p.N && first + j < end) o[(long long)j * p.ldo] = __float2bfloat16_rn(y);
+                        const float g = (float)__float_as_int(gate ? v[j] : u[j]) * (xs[j] * ws), up = (float)__float_as_int(gate ? u[j] : v[j]) * (xs[j] * ws2);
+                        v[j] = g, u[j] = up;
+                    }
+                    if (p.act == 0) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = i8_silu_times(v[j], u[j]);
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) {       // a loop over quarters: sixteen copies of the other gates' code do not fit the instruction cache
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float y = q6k_gated(v[j], u[j], p.act, p.act_param);
+                                v[j] = v[j + 4], v[j + 4] = v[j + 8], v[j + 8] = v[j + 12], v[j + 12] = y;
+                                u[j] = u[j + 4], u[j + 4] = u[j + 8], u[j + 8] = u[j + 12];
+                            }
+                        }
+                    }
+                    if (rows >= 16) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, o += p.ldo) *o = __float2bfloat16_rn(v[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, o += p.ldo)
+                            if (j < rows) *o = __float2bfloat16_rn(v[j]);
                     }
                 }
             } else {
 #pragma unroll 1
                 for (int c0 = 0; c0 < end; c0 += 16) {
-                    int v[16];
-                    tmem_ld16_ints(from + c0, v);
+                    float v[16];                         // 32-bit integers until they are scaled
+                    tmem_ld16_issue(from + c0, v);
+                    tmem_ld_wait();
                     if (c0 + 16 >= end) release();
-                    const float xs = next;
-                    next = row_scale(c0 + 16);
+                    float xs[16];
+                    scales_of(c0, xs);
+                    const int rows = n < p.N ? end - c0 : 0;
+                    const long long at = (long long)(row0 + c0) * p.ldo + n;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float f = (float)v[j] * (__shfl_sync(0xffffffffu, xs, j) * ws);
-                        if (n < p.N && c0 + j < end) {
-                            const long long at = (long long)(row0 + c0 + j) * p.ldo + n;
-                            if (p.epilogue == I8_ADD) atomicAdd((float*)p.out + at, f);      // nobody else adds here: one addition, without waiting for what is there
-                            else if (p.epilogue == I8_ACT) ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(q6k_activation(f, p.act));
-                            else ((float*)p.out)[at] = f;
+                    for (int j = 0; j < 16; ++j) v[j] = (float)__float_as_int(v[j]) * (xs[j] * ws);
+                    if (p.epilogue == I8_ACT) {
+                        __nv_bfloat16* o = (__nv_bfloat16*)p.out + at;
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i, o += p.ldo) {
+                            if (i < rows) *o = __float2bfloat16_rn(q6k_activation(v[0], p.act));
+#pragma unroll
+                            for (int j = 0; j < 15; ++j) v[j] = v[j + 1];
                         }
+                    } else if (p.epilogue == I8_ADD) {   // nobody else adds here: one addition each, without waiting for what is there
+                        float* o = (float*)p.out + at;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, o += p.ldo)
+                            if (j < rows) atomicAdd(o, v[j]);
+                    } else if (rows >= 16) {
+                        float* o = (float*)p.out + at;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, o += p.ldo) *o = v[j];
+                    } else {
+                        float* o = (float*)p.out + at;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, o += p.ldo)
+                            if (j < rows) *o = v[j];
                     }
                 }
             }
@@ -359,7 +402,7 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
     if (DUAL)
         if (int rc = make_i8_map(&tw2, p.w2, (long long)p.groups * p.N, p.K, p.K, w_box, true)) return rc;
     if (int rc = make_i8_map(&ta, p.a, a_total, p.K, p.lda, BT / CTAS, false)) return rc;
-    const int extra = (DUAL ? EW * SWAP_BYTES : 0) + (p.offsets ? (p.groups + 1) * 4 : 0);
+    const int extra = (DUAL ? EW * SWAP_BYTES : 0) + EW * SCALE_BYTES + (p.offsets ? (p.groups + 1) * 4 : 0);
     t.stages = (222 * 1024 - extra) / stage;
     if (t.stages > MAX_STAGES) t.stages = MAX_STAGES;
     t.n_x = (p.N + COLS - 1) / COLS, t.n_y = (p.rows + BT - 1) / BT;
