@@ -13,6 +13,7 @@ namespace {
 
 constexpr int SEL_THREADS = 256, SEL_MAX_COUNT = 256, SEL_MAX_WIDTH = 32;
 constexpr int SEL_EACH = 32, SEL_SLICE = SEL_THREADS * SEL_EACH;
+constexpr int SEL_WARPS = SEL_THREADS / 32, SEL_POOL = 1024;       // how many keys are ranked by counting
 
 // An order-preserving number of a finite logit, above 0; 0 for what is not finite.
 __device__ __forceinline__ unsigned finite_key(float v) {
@@ -33,7 +34,43 @@ __device__ __forceinline__ int block_count(int v, int* red) {
     __syncthreads();
     int t = 0;
 #pragma unroll
-    for (int w = 0; w < SEL_THREADS / 32; ++w) t += red[w];
+    for (int w = 0; w < SEL_WARPS; ++w) t += red[w];
+    return t;
+}
+
+// The best `count` of many keys without sorting them: a key that at least `count` others reach.  Every thread brings the largest of the
+// keys that it holds; each warp finds the ceil(count / warps)-th largest of its threads' keys, and the smallest of those is reached by
+// as many keys as are wanted (or is 0, where there are fewer).  The keys that reach it are few: they are collected and ranked.
+__device__ __forceinline__ unsigned warp_kth(unsigned mine, int k) {
+    unsigned m = 0;
+    for (; k > 0; --k) {
+        m = __reduce_max_sync(0xffffffffu, mine);
+        const unsigned who = __ballot_sync(0xffffffffu, mine == m);
+        if ((threadIdx.x & 31) == __ffs(who) - 1) mine = 0;
+        if (m == 0) break;
+    }
+    return m;
+}
+__device__ __forceinline__ unsigned long long warp_kth(unsigned long long mine, int k) {
+    unsigned long long m = 0;
+    for (; k > 0; --k) {
+        const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(mine >> 32));
+        const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(mine >> 32) == hi ? (unsigned)mine : 0u);
+        m = (unsigned long long)hi << 32 | lo;
+        const unsigned who = __ballot_sync(0xffffffffu, mine == m);
+        if ((threadIdx.x & 31) == __ffs(who) - 1) mine = 0;
+        if (m == 0) break;
+    }
+    return m;
+}
+template <typename K>
+__device__ __forceinline__ K block_threshold(K mine, int count, K* of_warp) {
+    const K m = warp_kth(mine, (count + SEL_WARPS - 1) / SEL_WARPS);
+    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = m;
+    __syncthreads();
+    K t = of_warp[0];
+#pragma unroll
+    for (int w = 1; w < SEL_WARPS; ++w) t = of_warp[w] < t ? of_warp[w] : t;
     return t;
 }
 
@@ -43,72 +80,100 @@ struct SliceHead {
     int found;
 };
 
-__global__ void __launch_bounds__(SEL_THREADS) beam_slice_kernel(const float* logits, int V, int count, float* best, int* at, SliceHead* heads) {
+// WIDE: rows start on 16 bytes.
+template <bool WIDE>
+__global__ void __launch_bounds__(SEL_THREADS, 4) beam_slice_kernel(const float* logits, int V, int count, float* best, int* at, SliceHead* heads) {
     pdl_enter();
-    __shared__ int red[SEL_THREADS / 32];
+    __shared__ int red[SEL_WARPS];
     __shared__ float redf[32];
+    __shared__ unsigned of_warp[SEL_WARPS];
+    __shared__ unsigned all[SEL_SLICE];                      // every key of the slice, where the pool is not enough
+    unsigned* key = all;
+    int* place = (int*)(all + SEL_POOL);
     __shared__ int taken;
     const float* row = logits + (size_t)blockIdx.y * V;
     const int lo = blockIdx.x * SEL_SLICE, n = min(V - lo, SEL_SLICE);
     const size_t slot = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
     float v[SEL_EACH];
+    auto where = [&](int j) { return WIDE ? (j >> 2) * (SEL_THREADS * 4) + (int)threadIdx.x * 4 + (j & 3) : j * SEL_THREADS + (int)threadIdx.x; };
+    if (WIDE) {
+#pragma unroll
+        for (int j = 0; j < SEL_EACH; j += 4) {
+            const float4 f = where(j) < n ? __ldcs((const float4*)(row + lo + where(j))) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);      // n is a multiple of 4
+            v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < SEL_EACH; ++j) v[j] = where(j) < n ? __ldcs(row + lo + where(j)) : -INFINITY;
+    }
     float most = -INFINITY;
+    unsigned mine = 0;
     bool bad = false;                                        // a value that makes the row's sum not finite
 #pragma unroll
     for (int j = 0; j < SEL_EACH; ++j) {
-        const int i = j * SEL_THREADS + threadIdx.x;
-        v[j] = i < n ? row[lo + i] : -INFINITY;
         most = fmaxf(most, v[j]);
         bad |= !(v[j] < INFINITY);
     }
+    mine = finite_key(most);                                 // rows with another value that is not finite take no part
+    if (threadIdx.x == 0) taken = 0;
+    const unsigned reach = max(block_threshold(mine, count, of_warp), 1u);
     most = warp_max(most);
     if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = most;
-    if (threadIdx.x == 0) taken = 0;
     const bool any_bad = __syncthreads_or(bad);
 #pragma unroll
-    for (int w = 0; w < SEL_THREADS / 32; ++w) most = fmaxf(most, redf[w]);
+    for (int w = 0; w < SEL_WARPS; ++w) most = fmaxf(most, redf[w]);
+    if (any_bad || most == -INFINITY) {
+        if (threadIdx.x == 0) heads[slot] = SliceHead{most, any_bad ? NAN : 0.0f, 0};
+        return;
+    }
     float sum = 0.0f;
-    if (most > -INFINITY && !any_bad) {
 #pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) sum += expf(v[j] - most);
+    for (int j = 0; j < SEL_EACH; ++j) {
+        sum += __expf(v[j] - most);
+        const unsigned k = finite_key(v[j]);
+        if (k >= reach) {
+            const int to = atomicAdd(&taken, 1);
+            if (to < SEL_POOL) key[to] = k, place[to] = where(j);
+        }
     }
     sum = block_sum(sum, redf);
-    // the count-th largest (logit, lowest place) of the slice, bit by bit
-    int finite = 0;
+    const int found = taken;
+    if (threadIdx.x == 0) heads[slot] = SliceHead{most, sum, min(count, found)};
+    if (found <= SEL_POOL) {
+        for (int i = threadIdx.x; i < found; i += SEL_THREADS) {
+            int rank = 0;
+            const unsigned k = key[i];
+            const int p = place[i];
+            for (int j = 0; j < found; ++j) rank += key[j] > k || (key[j] == k && place[j] < p);
+            if (rank < count) best[slot * count + rank] = row[lo + p], at[slot * count + rank] = lo + p;
+        }
+        return;
+    }
+    // too many equal ones (or an order that hides the best): the count-th largest (logit, lowest place) bit by bit
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < SEL_EACH; ++j) finite += finite_key(v[j]) != 0u;
-    finite = block_count(finite, red);
-    const int want = min(count, finite);
-    if (threadIdx.x == 0) heads[slot] = SliceHead{most, any_bad ? NAN : sum, any_bad ? 0 : want};
-    if (want == 0 || any_bad) return;
+    for (int j = 0; j < SEL_EACH; ++j) all[where(j)] = finite_key(v[j]);
+    if (threadIdx.x == 0) taken = 0;
+    __syncthreads();
+    auto how_many = [&](auto&& is) {
+        int c = 0;
+        for (int i = threadIdx.x; i < SEL_SLICE; i += SEL_THREADS) c += is(all[i], i);
+        return block_count(c, red);
+    };
     unsigned kth = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const unsigned trial = kth | (1u << bit);
-        int c = 0;
-#pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) c += finite_key(v[j]) >= trial;
-        if (block_count(c, red) >= want) kth = trial;
+        if (how_many([&](unsigned k, int) { return k >= trial; }) >= count) kth = trial;
     }
-    int above = 0;
-#pragma unroll
-    for (int j = 0; j < SEL_EACH; ++j) above += finite_key(v[j]) > kth;
-    above = block_count(above, red);
+    const int above = how_many([&](unsigned k, int) { return k > kth; });
     int last = 0;                                            // of the logits equal to it, those at places below `last` are taken
-    for (int step = SEL_SLICE; step > 0; step >>= 1) {
-        int c = 0;
-#pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) c += finite_key(v[j]) == kth && j * SEL_THREADS + (int)threadIdx.x < last + step;
-        if (block_count(c, red) <= want - above) last += step;
-    }
-#pragma unroll
-    for (int j = 0; j < SEL_EACH; ++j) {
-        const unsigned k = finite_key(v[j]);
-        const int i = j * SEL_THREADS + threadIdx.x;
-        if (k > kth || (k == kth && i < last)) {
+    for (int step = SEL_SLICE; step > 0; step >>= 1)
+        if (how_many([&](unsigned k, int i) { return k == kth && i < last + step; }) <= count - above) last += step;
+    for (int i = threadIdx.x; i < n; i += SEL_THREADS)
+        if (all[i] > kth || (all[i] == kth && i < last)) {
             const int to = atomicAdd(&taken, 1);
-            if (to < want) best[slot * count + to] = v[j], at[slot * count + to] = lo + i;
+            if (to < count) best[slot * count + to] = row[lo + i], at[slot * count + to] = lo + i;
         }
-    }
 }
 
 // grid: requests.
@@ -119,8 +184,8 @@ __global__ void __launch_bounds__(SEL_THREADS) beam_merge_kernel(const float* lo
     __shared__ double base[SEL_MAX_WIDTH];                   // the beam's score less the logarithm of its row's sum
     __shared__ bool dead[SEL_MAX_WIDTH];
     __shared__ int red[SEL_THREADS / 32];
-    __shared__ unsigned long long key[SEL_MAX_COUNT];
-    __shared__ int place[SEL_MAX_COUNT];
+    __shared__ unsigned long long of_warp[SEL_WARPS], key[SEL_POOL];
+    __shared__ int place[SEL_POOL];
     __shared__ int taken;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t row0 = (size_t)blockIdx.x * width;
@@ -151,59 +216,69 @@ __global__ void __launch_bounds__(SEL_THREADS) beam_merge_kernel(const float* lo
         k = score_key(base[b] + (double)best[i]), where = b * V + token;
         return true;
     };
+    unsigned long long mine = 0;
     int c = 0;
     for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
         unsigned long long k;
         int w;
-        c += candidate(i, k, w);
+        if (candidate(i, k, w)) mine = k > mine ? k : mine, ++c;
     }
     const int want = min(count, block_count(c, red));
-    unsigned long long kth = 0;
-    int last = 0;
+    const unsigned long long reach = block_threshold(mine, count, of_warp);
     if (want > 0) {
-        for (int bit = 63; bit >= 0; --bit) {
-            const unsigned long long trial = kth | (1ull << bit);
-            c = 0;
-            for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
-                unsigned long long k;
-                int w;
-                c += candidate(i, k, w) && k >= trial;
-            }
-            if (block_count(c, red) >= want) kth = trial;
-        }
-        int above = 0;
         for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
             unsigned long long k;
             int w;
-            above += candidate(i, k, w) && k > kth;
+            if (candidate(i, k, w) && k >= reach) {
+                const int to = atomicAdd(&taken, 1);
+                if (to < SEL_POOL) key[to] = k, place[to] = w;
+            }
         }
-        above = block_count(above, red);
-        for (int step = 1 << 30; step > 0; step >>= 1) {
+    }
+    __syncthreads();
+    int found = taken;
+    if (found > SEL_POOL) {                                  // as in the slices: the want-th largest (score, lowest place) bit by bit
+        auto how_many = [&](auto&& is) {
             c = 0;
             for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
                 unsigned long long k;
                 int w;
-                c += candidate(i, k, w) && k == kth && w < last + step;
+                c += candidate(i, k, w) && is(k, w);
             }
-            if (block_count(c, red) <= want - above) last += step;
+            return block_count(c, red);
+        };
+        unsigned long long kth = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const unsigned long long trial = kth | (1ull << bit);
+            if (how_many([&](unsigned long long k, int) { return k >= trial; }) >= want) kth = trial;
         }
+        const int above = how_many([&](unsigned long long k, int) { return k > kth; });
+        int last = 0;
+        for (int step = 1 << 30; step > 0; step >>= 1)
+            if (how_many([&](unsigned long long k, int w) { return k == kth && w < last + step; }) <= want - above) last += step;
+        __syncthreads();
+        if (threadIdx.x == 0) taken = 0;
+        __syncthreads();
         for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
             unsigned long long k;
             int w;
             if (candidate(i, k, w) && (k > kth || (k == kth && w < last))) {
                 const int to = atomicAdd(&taken, 1);
-                if (to < want) key[to] = k, place[to] = w;
+                if (to < SEL_POOL) key[to] = k, place[to] = w;
             }
         }
+        __syncthreads();
+        found = min(taken, SEL_POOL);
     }
-    __syncthreads();
     out_score += (size_t)blockIdx.x * count, out_beam += (size_t)blockIdx.x * count, out_token += (size_t)blockIdx.x * count;
-    for (int i = threadIdx.x; i < want; i += SEL_THREADS) {
+    for (int i = threadIdx.x; i < found; i += SEL_THREADS) {
         int rank = 0;
-        for (int j = 0; j < want; ++j) rank += key[j] > key[i] || (key[j] == key[i] && place[j] < place[i]);
         const unsigned long long u = key[i];
+        const int w = place[i];
+        for (int j = 0; j < found; ++j) rank += key[j] > u || (key[j] == u && place[j] < w);
+        if (rank >= want) continue;
         out_score[rank] = (float)__longlong_as_double((long long)((u >> 63) ? u & ~(1ull << 63) : ~u));
-        out_beam[rank] = place[i] / V, out_token[rank] = place[i] % V;
+        out_beam[rank] = w / V, out_token[rank] = w % V;
     }
     // fewer finite continuations than wanted (every one of them is listed): the others in order of place
     if (warp == 0) {
@@ -243,7 +318,8 @@ Q6K_API int q6k_beam_select(const float* logits, const float* scores, int reques
     float* best = (float*)scratch;
     int* at = (int*)(best + (size_t)rows * slices * count);
     SliceHead* heads = (SliceHead*)(at + (size_t)rows * slices * count);
-    q6k_launch(beam_slice_kernel, dim3(slices, rows), SEL_THREADS, 0, st, logits, V, count, best, at, heads);
-    q6k_launch(beam_merge_kernel, requests, SEL_THREADS, 0, st, logits, scores, V, width, slices, count, best, at, heads, out_score, out_beam, out_token);
+    if (V % 4 == 0 && ((uintptr_t)logits & 15) == 0) q6k_launch(beam_slice_kernel<true>, dim3(slices, rows), SEL_THREADS, 0, st, logits, V, count, best, at, heads);
+    else q6k_launch(beam_slice_kernel<false>, dim3(slices, rows), SEL_THREADS, 0, st, logits, V, count, best, at, heads);
+    q6k_launch_as(true, beam_merge_kernel, requests, SEL_THREADS, 0, st, logits, scores, V, width, slices, count, best, at, heads, out_score, out_beam, out_token);
     return q6k_check_launch("beam_select");
 }
