@@ -3,17 +3,22 @@
 // over all beams b and tokens v, in descending order, the lowest place b V + v first among equals.  A continuation whose beam's
 // score, logit or sum is not finite counts as -infinity: it comes after every other one, in order of place.
 //
-// Logits are read once.  A block takes a slice of one row and leaves the slice's maximum, its sum of exponentials over that
+// Logits are read once.  A block takes a part of one row and leaves the part's maximum, its sum of exponentials over that
 // maximum, and its `count` best logits (within a row the order of the logits is the order of t).  A block per request then
-// makes the rows' sums and finds the best of what the slices left.  t is compared in 64 bits: two logits of one row that differ
+// makes the rows' sums and finds the best of what the parts left.  t is compared in 64 bits: two logits of one row that differ
 // give scores that differ, and scores of different beams are not made equal by a rounding.
-#include "common.cuh"
+#include <cfloat>
+
+#include "umma.cuh"
 
 namespace {
 
-constexpr int SEL_THREADS = 256, SEL_MAX_COUNT = 256, SEL_MAX_WIDTH = 32;
-constexpr int SEL_EACH = 32, SEL_SLICE = SEL_THREADS * SEL_EACH;
-constexpr int SEL_WARPS = SEL_THREADS / 32, SEL_POOL = 1024;       // how many keys are ranked by counting
+constexpr int SEL_THREADS = 256, SEL_MAX_COUNT = 128, SEL_MAX_WIDTH = 32;
+constexpr int SEL_EACH = 32, SEL_TILE = SEL_THREADS * SEL_EACH;
+constexpr int MERGE_THREADS = 512, MERGE_WARPS = MERGE_THREADS / 32;
+constexpr int SEL_WARPS = SEL_THREADS / 32, SEL_POOL = 1024, SEL_TILES = 8;       // keys that a pool holds; the most tiles of a part
+constexpr int SEL_PARTS = 4;       // parts to an SM that a long batch is cut into (8: 29 us where 4 take 25, 128 rows of 151,936 logits: more parts leave more to merge)
+constexpr float LOG2E = 1.4426950408889634f;
 
 // An order-preserving number of a finite logit, above 0; 0 for what is not finite.
 __device__ __forceinline__ unsigned finite_key(float v) {
@@ -21,12 +26,14 @@ __device__ __forceinline__ unsigned finite_key(float v) {
     if ((u & 0x7fffffffu) >= 0x7f800000u) return 0u;
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k); }
 // The same for a score in 64 bits (finite by construction).
 __device__ __forceinline__ unsigned long long score_key(double v) {
     const unsigned long long u = (unsigned long long)__double_as_longlong(v == 0.0 ? 0.0 : v);
     return (u >> 63) ? ~u : (u | (1ull << 63));
 }
 
+template <int WARPS>
 __device__ __forceinline__ int block_count(int v, int* red) {
     v = __reduce_add_sync(0xffffffffu, v);
     __syncthreads();
@@ -34,131 +41,131 @@ __device__ __forceinline__ int block_count(int v, int* red) {
     __syncthreads();
     int t = 0;
 #pragma unroll
-    for (int w = 0; w < SEL_WARPS; ++w) t += red[w];
+    for (int w = 0; w < WARPS; ++w) t += red[w];
     return t;
 }
 
-// The best `count` of many keys without sorting them: a key that at least `count` others reach.  Every thread brings the largest of the
-// keys that it holds; each warp finds the ceil(count / warps)-th largest of its threads' keys, and the smallest of those is reached by
-// as many keys as are wanted (or is 0, where there are fewer).  The keys that reach it are few: they are collected and ranked.
-__device__ __forceinline__ unsigned warp_kth(unsigned mine, int k) {
-    unsigned m = 0;
-    for (; k > 0; --k) {
-        m = __reduce_max_sync(0xffffffffu, mine);
-        const unsigned who = __ballot_sync(0xffffffffu, mine == m);
-        if ((threadIdx.x & 31) == __ffs(who) - 1) mine = 0;
-        if (m == 0) break;
+// The best `count` of many keys without sorting them: a number that at least `count` of them reach and few others do.  Every thread brings the largest
+// of the keys that it holds; the count-th largest of those is found from its highest bit down, and no further than until few more reach it than are
+// wanted.  0: fewer than `count` threads hold any.
+__device__ __forceinline__ unsigned block_threshold(unsigned mine, int count) {
+    unsigned t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned trial = t | (1u << bit);
+        const int c = __syncthreads_count(mine >= trial);
+        if (c >= count) t = trial;
+        if (c >= count && c <= count + count / 4) break;
     }
-    return m;
-}
-__device__ __forceinline__ unsigned long long warp_kth(unsigned long long mine, int k) {
-    unsigned long long m = 0;
-    for (; k > 0; --k) {
-        const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(mine >> 32));
-        const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(mine >> 32) == hi ? (unsigned)mine : 0u);
-        m = (unsigned long long)hi << 32 | lo;
-        const unsigned who = __ballot_sync(0xffffffffu, mine == m);
-        if ((threadIdx.x & 31) == __ffs(who) - 1) mine = 0;
-        if (m == 0) break;
-    }
-    return m;
-}
-template <typename K>
-__device__ __forceinline__ K block_threshold(K mine, int count, K* of_warp) {
-    const K m = warp_kth(mine, (count + SEL_WARPS - 1) / SEL_WARPS);
-    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = m;
-    __syncthreads();
-    K t = of_warp[0];
-#pragma unroll
-    for (int w = 1; w < SEL_WARPS; ++w) t = of_warp[w] < t ? of_warp[w] : t;
     return t;
 }
 
-// grid (slices, rows).  best/at: [rows, slices, count]; head: [rows, slices] of {maximum, sum, how many}.
-struct SliceHead {
+// What a part of a row leaves: its maximum and its sum of exponentials over that maximum.
+struct PartHead {
     float most, sum;
-    int found;
 };
 
-// WIDE: rows start on 16 bytes.
+// grid (parts, rows); a part is `tiles` tiles of 8,192 logits.  best/at: [rows, parts, count] (at -1: none); heads: [rows, parts].  WIDE: rows start
+// on 16 bytes.  The pass over the logits keeps each thread's maximum of every tile and its sum, and nothing in it waits for another warp.  The threads'
+// maxima give the threshold; the few (thread, tile) pieces that reach it are read again, a warp each.
 template <bool WIDE>
-__global__ void __launch_bounds__(SEL_THREADS, 4) beam_slice_kernel(const float* logits, int V, int count, float* best, int* at, SliceHead* heads) {
+__global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* logits, int V, int tiles, int count, float* best, int* at, PartHead* heads) {
     pdl_enter();
     __shared__ int red[SEL_WARPS];
-    __shared__ float redf[32];
-    __shared__ unsigned of_warp[SEL_WARPS];
-    __shared__ unsigned all[SEL_SLICE];                      // every key of the slice, where the pool is not enough
-    unsigned* key = all;
-    int* place = (int*)(all + SEL_POOL);
-    __shared__ int taken;
+    __shared__ float redf[32], redm[SEL_WARPS];
+    __shared__ unsigned key[SEL_POOL];
+    __shared__ int place[SEL_POOL];
+    __shared__ float piece_most[SEL_TILES][SEL_THREADS];
+    __shared__ unsigned short pieces[SEL_TILES * SEL_THREADS];
+    __shared__ int taken, listed;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* row = logits + (size_t)blockIdx.y * V;
-    const int lo = blockIdx.x * SEL_SLICE, n = min(V - lo, SEL_SLICE);
+    const int lo = blockIdx.x * tiles * SEL_TILE, hi = (int)min((long long)V, (long long)lo + (long long)tiles * SEL_TILE);
     const size_t slot = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
-    float v[SEL_EACH];
-    auto where = [&](int j) { return WIDE ? (j >> 2) * (SEL_THREADS * 4) + (int)threadIdx.x * 4 + (j & 3) : j * SEL_THREADS + (int)threadIdx.x; };
-    if (WIDE) {
+    best += slot * count, at += slot * count;
+    auto where = [](int thread, int j) { return WIDE ? (j >> 2) * (SEL_THREADS * 4) + thread * 4 + (j & 3) : j * SEL_THREADS + thread; };
+    float most = -INFINITY, sum = 0.0f;                      // of this thread (a NaN is passed over by the maxima and found again in the sum)
+    if (threadIdx.x == 0) taken = 0, listed = 0;
+    for (int t = 0; t < tiles && lo + t * SEL_TILE < hi; ++t) {
+        const int n = hi - lo - t * SEL_TILE;                // (WIDE: a multiple of 4)
+        const float* tile = row + lo + t * SEL_TILE;
+        float v[SEL_EACH];
+        if (WIDE) {
 #pragma unroll
-        for (int j = 0; j < SEL_EACH; j += 4) {
-            const float4 f = where(j) < n ? __ldcs((const float4*)(row + lo + where(j))) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);      // n is a multiple of 4
-            v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+            for (int j = 0; j < SEL_EACH; j += 4) {
+                const int i = where(threadIdx.x, j);
+                const float4 f = i < n ? __ldg((const float4*)(tile + i)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < SEL_EACH; ++j) v[j] = where(threadIdx.x, j) < n ? __ldg(tile + where(threadIdx.x, j)) : -INFINITY;
         }
-    } else {
+        float high = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) v[j] = where(j) < n ? __ldcs(row + lo + where(j)) : -INFINITY;
-    }
-    float most = -INFINITY;
-    unsigned mine = 0;
-    bool bad = false;                                        // a value that makes the row's sum not finite
+        for (int j = 0; j < SEL_EACH; ++j) high = fmaxf(high, v[j]);
+        piece_most[t][threadIdx.x] = high;
+        const float m = fmaxf(most, high);
+        if (m > -INFINITY) {
+            // 2^(x L - c) with c = m L rounded: the rounding of c multiplies the whole sum by 2^d, d = m L - c, which is known exactly
+            const float c = m * LOG2E, d = fmaf(m, LOG2E, -c);
+            float here = 0.0f;
+            if (fabsf(m) < 1e30f) {
 #pragma unroll
-    for (int j = 0; j < SEL_EACH; ++j) {
-        most = fmaxf(most, v[j]);
-        bad |= !(v[j] < INFINITY);
-    }
-    mine = finite_key(most);                                 // rows with another value that is not finite take no part
-    if (threadIdx.x == 0) taken = 0;
-    const unsigned reach = max(block_threshold(mine, count, of_warp), 1u);
-    most = warp_max(most);
-    if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = most;
-    const bool any_bad = __syncthreads_or(bad);
+                for (int j = 0; j < SEL_EACH; ++j) here += ex2_approx(fmaf(v[j], LOG2E, -c));
+                here *= ex2_approx(-d);
+            } else {                                         // m L may be infinite
 #pragma unroll
-    for (int w = 0; w < SEL_WARPS; ++w) most = fmaxf(most, redf[w]);
-    if (any_bad || most == -INFINITY) {
-        if (threadIdx.x == 0) heads[slot] = SliceHead{most, any_bad ? NAN : 0.0f, 0};
-        return;
-    }
-    float sum = 0.0f;
+                for (int j = 0; j < SEL_EACH; ++j) here += ex2_approx((v[j] - m) * LOG2E);
+            }
+            sum = sum * ex2_approx((most - m) * LOG2E) + here;
+            most = m;
+        } else {
 #pragma unroll
-    for (int j = 0; j < SEL_EACH; ++j) {
-        sum += __expf(v[j] - most);
-        const unsigned k = finite_key(v[j]);
-        if (k >= reach) {
-            const int to = atomicAdd(&taken, 1);
-            if (to < SEL_POOL) key[to] = k, place[to] = where(j);
+            for (int j = 0; j < SEL_EACH; ++j)
+                if (!(v[j] == -INFINITY)) sum = NAN;         // nothing but NaNs
         }
     }
+    float block_most = warp_max(most);
+    if (lane == 0) redm[warp] = block_most;
+    const unsigned low = block_threshold(finite_key(most), count);
+    const float reach = low != 0 ? key_value(low) : -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < SEL_WARPS; ++w) block_most = fmaxf(block_most, redm[w]);
+    for (int t = 0; t < tiles && lo + t * SEL_TILE < hi; ++t)
+        if (piece_most[t][threadIdx.x] >= reach && most < INFINITY) pieces[atomicAdd(&listed, 1)] = (unsigned short)(t * SEL_THREADS + threadIdx.x);
+    if (most > -INFINITY) sum *= ex2_approx((most - block_most) * LOG2E);
     sum = block_sum(sum, redf);
+    if (threadIdx.x == 0) heads[slot] = PartHead{block_most, sum};
+    for (int i = warp; i < listed; i += SEL_WARPS) {
+        const int t = pieces[i] / SEL_THREADS, p = lo + t * SEL_TILE + where(pieces[i] % SEL_THREADS, lane);
+        const float v = p < hi ? row[p] : -INFINITY;
+        const bool mine = v >= reach;
+        const unsigned who = __ballot_sync(0xffffffffu, mine);
+        int to = 0;
+        if (lane == 0) to = atomicAdd(&taken, __popc(who));
+        to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1u));
+        if (mine && to < SEL_POOL) key[to] = finite_key(v), place[to] = p;
+    }
+    __syncthreads();
     const int found = taken;
-    if (threadIdx.x == 0) heads[slot] = SliceHead{most, sum, min(count, found)};
     if (found <= SEL_POOL) {
         for (int i = threadIdx.x; i < found; i += SEL_THREADS) {
             int rank = 0;
             const unsigned k = key[i];
             const int p = place[i];
             for (int j = 0; j < found; ++j) rank += key[j] > k || (key[j] == k && place[j] < p);
-            if (rank < count) best[slot * count + rank] = row[lo + p], at[slot * count + rank] = lo + p;
+            if (rank < count) best[rank] = key_value(k), at[rank] = p;
         }
+        for (int i = found + threadIdx.x; i < count; i += SEL_THREADS) at[i] = -1;
         return;
     }
     // too many equal ones (or an order that hides the best): the count-th largest (logit, lowest place) bit by bit
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SEL_EACH; ++j) all[where(j)] = finite_key(v[j]);
     if (threadIdx.x == 0) taken = 0;
-    __syncthreads();
     auto how_many = [&](auto&& is) {
         int c = 0;
-        for (int i = threadIdx.x; i < SEL_SLICE; i += SEL_THREADS) c += is(all[i], i);
-        return block_count(c, red);
+        for (int i = lo + threadIdx.x; i < hi; i += SEL_THREADS) c += is(finite_key(row[i]), i);
+        return block_count<SEL_WARPS>(c, red);
     };
     unsigned kth = 0;
     for (int bit = 31; bit >= 0; --bit) {
@@ -167,85 +174,82 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_slice_kernel(const float*
     }
     const int above = how_many([&](unsigned k, int) { return k > kth; });
     int last = 0;                                            // of the logits equal to it, those at places below `last` are taken
-    for (int step = SEL_SLICE; step > 0; step >>= 1)
+    for (int step = 1 << 30; step > 0; step >>= 1)
         if (how_many([&](unsigned k, int i) { return k == kth && i < last + step; }) <= count - above) last += step;
-    for (int i = threadIdx.x; i < n; i += SEL_THREADS)
-        if (all[i] > kth || (all[i] == kth && i < last)) {
+    for (int i = lo + threadIdx.x; i < hi; i += SEL_THREADS) {
+        const unsigned k = finite_key(row[i]);
+        if (k > kth || (k == kth && i < last)) {
             const int to = atomicAdd(&taken, 1);
-            if (to < count) best[slot * count + to] = row[lo + i], at[slot * count + to] = lo + i;
+            if (to < count) best[to] = row[i], at[to] = i;
         }
+    }
 }
 
 // grid: requests.
-__global__ void __launch_bounds__(SEL_THREADS) beam_merge_kernel(const float* logits, const float* scores, int V, int width, int slices, int count,
-                                                                 const float* best, const int* at, const SliceHead* heads, float* out_score, int* out_beam,
+__global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(const float* logits, const float* scores, int V, int width, int parts, int count,
+                                                                 const float* best, const int* at, const PartHead* heads, float* out_score, int* out_beam,
                                                                  int* out_token) {
     pdl_enter();
-    __shared__ double base[SEL_MAX_WIDTH];                   // the beam's score less the logarithm of its row's sum
+    __shared__ double base[SEL_MAX_WIDTH], row_most[SEL_MAX_WIDTH];      // the beam's score less the logarithm of its row's sum over the row's maximum
     __shared__ bool dead[SEL_MAX_WIDTH];
-    __shared__ int red[SEL_THREADS / 32];
-    __shared__ unsigned long long of_warp[SEL_WARPS], key[SEL_POOL];
+    __shared__ int red[MERGE_THREADS / 32];
+    __shared__ unsigned long long key[SEL_POOL];
     __shared__ int place[SEL_POOL];
     __shared__ int taken;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t row0 = (size_t)blockIdx.x * width;
-    heads += row0 * slices, best += row0 * slices * count, at += row0 * slices * count, scores += row0;
-    for (int b = warp; b < width; b += SEL_THREADS / 32) {
+    heads += row0 * parts, best += row0 * parts * count, at += row0 * parts * count, scores += row0;
+    for (int b = warp; b < width; b += MERGE_WARPS) {
+        const float score = scores[b];
         float most = -INFINITY;
-        for (int s = lane; s < slices; s += 32) most = fmaxf(most, heads[b * slices + s].most);
-        most = warp_max(most);
-        double sum = 0.0;
-        for (int s = lane; s < slices; s += 32) {
-            const SliceHead h = heads[b * slices + s];
-            if (!(h.sum == 0.0f)) sum += (double)h.sum * exp((double)h.most - (double)most);
+        double sum = 0.0;                                    // over `most`
+        for (int s = lane; s < parts; s += 32) {
+            const PartHead h = heads[b * parts + s];
+            if (h.sum == 0.0f) continue;                     // nothing finite
+            const float m = fmaxf(most, h.most);
+            sum = sum * expf(most - m) + (double)h.sum * expf(h.most - m);       // one of the two exponents is 0
+            most = m;
         }
+        const float all_most = warp_max(most);
+        if (sum != 0.0) sum *= expf(most - all_most);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
-            const double d = (double)scores[b] - ((double)most + log(sum));
-            base[b] = d, dead[b] = !(fabs(d) < INFINITY);
+            const double d = (double)score - log(sum);
+            base[b] = d, row_most[b] = (double)all_most, dead[b] = !(fabs(d) < INFINITY && fabsf(all_most) < INFINITY);
         }
     }
     if (threadIdx.x == 0) taken = 0;
     __syncthreads();
-    const int per_row = slices * count, all = width * per_row;
-    auto candidate = [&](int i, unsigned long long& k, int& where) {
-        const int b = i / per_row, s = i / count % slices;
-        if (dead[b] || i % count >= heads[b * slices + s].found) return false;
-        const int token = at[i];
-        k = score_key(base[b] + (double)best[i]), where = b * V + token;
-        return true;
+    const int per_row = parts * count, all = width * per_row;
+    const float inverse = 1.0f / (float)per_row;
+    auto each = [&](auto&& f) {                              // every candidate; the rows are spread over all threads
+        for (int i = threadIdx.x; i < all; i += MERGE_THREADS) {
+            const int token = at[i];
+            int b = (int)((float)i * inverse);
+            b -= b * per_row > i, b += (b + 1) * per_row <= i;
+            if (token >= 0 && !dead[b]) f(score_key(base[b] + ((double)best[i] - row_most[b])), b * V + token);
+        }
     };
     unsigned long long mine = 0;
     int c = 0;
-    for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
-        unsigned long long k;
-        int w;
-        if (candidate(i, k, w)) mine = k > mine ? k : mine, ++c;
-    }
-    const int want = min(count, block_count(c, red));
-    const unsigned long long reach = block_threshold(mine, count, of_warp);
-    if (want > 0) {
-        for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
-            unsigned long long k;
-            int w;
-            if (candidate(i, k, w) && k >= reach) {
-                const int to = atomicAdd(&taken, 1);
-                if (to < SEL_POOL) key[to] = k, place[to] = w;
-            }
-        }
-    }
+    each([&](unsigned long long k, int) { mine = k > mine ? k : mine, ++c; });
+    const int want = min(count, block_count<MERGE_WARPS>(c, red));
+    const unsigned long long reach = (unsigned long long)block_threshold((unsigned)(mine >> 32), count) << 32;
+    auto take = [&](unsigned long long k, int w) {
+        const int to = atomicAdd(&taken, 1);
+        if (to < SEL_POOL) key[to] = k, place[to] = w;
+    };
+    each([&](unsigned long long k, int w) {
+        if (k >= reach) take(k, w);
+    });
     __syncthreads();
     int found = taken;
-    if (found > SEL_POOL) {                                  // as in the slices: the want-th largest (score, lowest place) bit by bit
+    if (found > SEL_POOL) {                                  // as in the parts: the want-th largest (score, lowest place) bit by bit
         auto how_many = [&](auto&& is) {
             c = 0;
-            for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
-                unsigned long long k;
-                int w;
-                c += candidate(i, k, w) && is(k, w);
-            }
-            return block_count(c, red);
+            each([&](unsigned long long k, int w) { c += is(k, w); });
+            return block_count<MERGE_WARPS>(c, red);
         };
         unsigned long long kth = 0;
         for (int bit = 63; bit >= 0; --bit) {
@@ -259,19 +263,14 @@ __global__ void __launch_bounds__(SEL_THREADS) beam_merge_kernel(const float* lo
         __syncthreads();
         if (threadIdx.x == 0) taken = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < all; i += SEL_THREADS) {
-            unsigned long long k;
-            int w;
-            if (candidate(i, k, w) && (k > kth || (k == kth && w < last))) {
-                const int to = atomicAdd(&taken, 1);
-                if (to < SEL_POOL) key[to] = k, place[to] = w;
-            }
-        }
+        each([&](unsigned long long k, int w) {
+            if (k > kth || (k == kth && w < last)) take(k, w);
+        });
         __syncthreads();
         found = min(taken, SEL_POOL);
     }
     out_score += (size_t)blockIdx.x * count, out_beam += (size_t)blockIdx.x * count, out_token += (size_t)blockIdx.x * count;
-    for (int i = threadIdx.x; i < found; i += SEL_THREADS) {
+    for (int i = threadIdx.x; i < found; i += MERGE_THREADS) {
         int rank = 0;
         const unsigned long long u = key[i];
         const int w = place[i];
@@ -295,7 +294,16 @@ __global__ void __launch_bounds__(SEL_THREADS) beam_merge_kernel(const float* lo
     }
 }
 
-int sel_slices(int V) { return (V + SEL_SLICE - 1) / SEL_SLICE; }
+// Tiles of a part: as many as leave some four parts to an SM (which run at a time).
+int part_tiles(long long rows, int V) {
+    const int tiles = (V + SEL_TILE - 1) / SEL_TILE, most = tiles < SEL_TILES ? tiles : SEL_TILES;
+    const long long each = (rows * tiles + SEL_PARTS * 148 - 1) / (SEL_PARTS * 148);
+    return (int)(each < 1 ? 1 : each < most ? each : most);
+}
+int row_parts(long long rows, int V) {
+    const int tiles = (V + SEL_TILE - 1) / SEL_TILE, each = part_tiles(rows, V);
+    return (tiles + each - 1) / each;
+}
 
 }  // namespace
 
@@ -303,7 +311,7 @@ Q6K_API int q6k_beam_max_count() { return SEL_MAX_COUNT; }
 Q6K_API int q6k_beam_max_width() { return SEL_MAX_WIDTH; }
 // Bytes of scratch that q6k_beam_select takes.
 Q6K_API long long q6k_beam_scratch(int rows, int V, int count) {
-    return (long long)rows * sel_slices(V) * ((long long)count * 8 + (long long)sizeof(SliceHead));
+    return (long long)rows * row_parts(rows, V) * ((long long)count * 8 + (long long)sizeof(PartHead));
 }
 
 // logits: FP32 [requests * width, V]; scores: FP32 [requests, width]; out_*: [requests, count].
@@ -313,13 +321,13 @@ Q6K_API int q6k_beam_select(const float* logits, const float* scores, int reques
     Q6K_REQUIRE(requests > 0 && requests * (long long)width <= 65535 && width >= 1 && width <= SEL_MAX_WIDTH && V >= 1 && (long long)width * V < (1LL << 31),
                 "beam_select: %d requests of %d beams over %d tokens", requests, width, V);
     Q6K_REQUIRE(count >= 1 && count <= SEL_MAX_COUNT && count <= (long long)width * V, "beam_select: %d continuations of %d beams over %d tokens", count, width, V);
-    const int rows = requests * width, slices = sel_slices(V);
+    const int rows = requests * width, tiles = part_tiles(rows, V), parts = row_parts(rows, V);
     Q6K_REQUIRE(scratch_bytes >= q6k_beam_scratch(rows, V, count), "beam_select: %lld bytes of scratch, %lld are needed", scratch_bytes, q6k_beam_scratch(rows, V, count));
     float* best = (float*)scratch;
-    int* at = (int*)(best + (size_t)rows * slices * count);
-    SliceHead* heads = (SliceHead*)(at + (size_t)rows * slices * count);
-    if (V % 4 == 0 && ((uintptr_t)logits & 15) == 0) q6k_launch(beam_slice_kernel<true>, dim3(slices, rows), SEL_THREADS, 0, st, logits, V, count, best, at, heads);
-    else q6k_launch(beam_slice_kernel<false>, dim3(slices, rows), SEL_THREADS, 0, st, logits, V, count, best, at, heads);
-    q6k_launch_as(true, beam_merge_kernel, requests, SEL_THREADS, 0, st, logits, scores, V, width, slices, count, best, at, heads, out_score, out_beam, out_token);
+    int* at = (int*)(best + (size_t)rows * parts * count);
+    PartHead* heads = (PartHead*)(at + (size_t)rows * parts * count);
+    if (V % 4 == 0 && ((uintptr_t)logits & 15) == 0) q6k_launch(beam_part_kernel<true>, dim3(parts, rows), SEL_THREADS, 0, st, logits, V, tiles, count, best, at, heads);
+    else q6k_launch(beam_part_kernel<false>, dim3(parts, rows), SEL_THREADS, 0, st, logits, V, tiles, count, best, at, heads);
+    q6k_launch_as(true, beam_merge_kernel, requests, MERGE_THREADS, 0, st, logits, scores, V, width, parts, count, best, at, heads, out_score, out_beam, out_token);
     return q6k_check_launch("beam_select");
 }

@@ -2,14 +2,14 @@
 // at once (a row may be the parent of others and have another parent itself).  Two forms of what a row holds: positions of paged
 // tensors, reached through a block table, and slots of fixed-size states.
 //
-// A thread owns one place (16 bytes of one position's row, or of one state) in all rows of a group: it reads the parents'
-// values of every row that moves, and writes them after the last read.  So no second copy is needed whatever the parents are,
+// A thread owns one place (16 bytes of a position's row, or of a state) in all rows of a group: it reads the parents' values
+// for every row that moves, and writes them after the last read.  So no second copy is needed whatever the parents are,
 // and nothing is synchronised.  All tensors of a call are handled by one launch.
 #include "common.cuh"
 
 namespace {
 
-constexpr int RE_TENSORS = 128, RE_MAX_WIDTH = 32, RE_THREADS = 256;
+constexpr int RE_TENSORS = 128, RE_MAX_WIDTH = 32, RE_THREADS = 256, RE_PIECE = 4096;
 
 struct PageTensors {                       // [heads, pages, page_size, a row of row_bytes]
     char* base[RE_TENSORS];
@@ -27,13 +27,16 @@ __device__ __forceinline__ int parent_of(const int* parents, int group, int widt
     return (unsigned)p < (unsigned)width ? p : b;
 }
 
-// grid (blocks along the places, tensors, groups); V: what a thread moves at a time; W: the most rows of a group.
-template <typename V, int W>
-__global__ void __launch_bounds__(RE_THREADS) reorder_pages_kernel(const __grid_constant__ PageTensors t, const int* table, int blocks, int page_size, const int* parents,
+// A warp works on a piece of up to RE_PIECE bytes of one head's part of one page, in all rows of a group: there the positions lie one after the other,
+// so that which bytes a row takes over are two numbers.  grid (blocks along the pieces, tensors, groups); V: what a lane moves at a time; W: the most rows
+// of a group; U: places that a lane has under way at once.
+// (A thread for each place, which found its page and row by divisions of its own, held 150 registers: 163 us for 262 MB where this takes 60.)
+template <typename V, int W, int U>
+__global__ void __launch_bounds__(RE_THREADS, W <= 8 ? 3 : 1) reorder_pages_kernel(const __grid_constant__ PageTensors t, const int* table, int blocks, int page_size, const int* parents,
                                                                    const int* first, const int* lengths, int width) {
     pdl_enter();
     __shared__ int par[RE_MAX_WIDTH], from[RE_MAX_WIDTH], to[RE_MAX_WIDTH];
-    const int group = blockIdx.z, row0 = group * width;
+    const int group = blockIdx.z, row0 = group * width, lane = threadIdx.x & 31;
     if (threadIdx.x < width) {
         const int b = threadIdx.x, p = parent_of(parents, group, width, b);
         par[b] = p, from[b] = max(first[row0 + b], 0), to[b] = p == b ? 0 : (int)min((long long)lengths[row0 + p], (long long)blocks * page_size);
@@ -44,30 +47,54 @@ __global__ void __launch_bounds__(RE_THREADS) reorder_pages_kernel(const __grid_
         if (from[b] < to[b]) lo = min(lo, from[b]), hi = max(hi, to[b]);
     if (lo >= hi) return;
     char* base = t.base[blockIdx.y];
-    const int heads = t.heads[blockIdx.y], pages = t.pages[blockIdx.y], vecs = t.row_bytes[blockIdx.y] / (int)sizeof(V);
-    const long long page_bytes = (long long)page_size * t.row_bytes[blockIdx.y];
-    const long long places = (long long)(hi - lo) * heads * vecs;
-    for (long long i = (long long)blockIdx.x * RE_THREADS + threadIdx.x; i < places; i += (long long)gridDim.x * RE_THREADS) {
-        const int vec = (int)(i % vecs), head = (int)(i / vecs % heads), pos = lo + (int)(i / vecs / heads);
-        const int block = pos / page_size;
-        const long long in_page = (long long)(pos % page_size) * t.row_bytes[blockIdx.y] + (long long)vec * sizeof(V);
-        auto where = [&](int b) -> V* {
-            const int page = table[(long long)(row0 + b) * blocks + block];
-            return (unsigned)page < (unsigned)pages ? (V*)(base + ((long long)head * pages + page) * page_bytes + in_page) : nullptr;
-        };
-        V held[W];
-        V* dst[W];
-#pragma unroll
-        for (int b = 0; b < W; ++b) {
-            dst[b] = nullptr;
-            if (b < width && pos >= from[b] && pos < to[b]) {
-                const V* src = where(par[b]);
-                if (src) held[b] = *src, dst[b] = where(b);
-            }
+    const unsigned heads = t.heads[blockIdx.y], pages = t.pages[blockIdx.y], row_bytes = t.row_bytes[blockIdx.y];
+    const long long page_bytes = (long long)page_size * row_bytes;
+    const unsigned per_page = (unsigned)((page_bytes + RE_PIECE - 1) / RE_PIECE);
+    const int block0 = lo / page_size, block1 = (hi - 1) / page_size + 1;
+    const long long pieces = (long long)(block1 - block0) * heads * per_page;
+    for (long long piece = (long long)blockIdx.x * (RE_THREADS / 32) + (threadIdx.x >> 5); piece < pieces; piece += (long long)gridDim.x * (RE_THREADS / 32)) {
+        const unsigned head = (unsigned)(piece / per_page % heads);
+        const int block = block0 + (int)(piece / per_page / heads);
+        const long long begin = piece % per_page * RE_PIECE, end = min(begin + RE_PIECE, page_bytes);
+        // lane b: row b's pages here (its parent's and its own), and which bytes of the piece it takes over
+        int src = -1, dst = -1, f = 0, e = 0;
+        if (lane < width && from[lane] < to[lane]) {
+            src = table[(size_t)(row0 + par[lane]) * blocks + block], dst = table[(size_t)(row0 + lane) * blocks + block];
+            const long long at = (long long)block * page_size;
+            f = (int)(min(max((from[lane] - at) * row_bytes, begin), end) - begin), e = (int)(min(max((to[lane] - at) * row_bytes, begin), end) - begin);
         }
+        unsigned moving = __ballot_sync(0xffffffffu, (unsigned)src < pages && (unsigned)dst < pages && f < e);
+        if (moving == 0) continue;
+        const V* from_page[W];
+        V* to_page[W];
+        int f_of[W], e_of[W];
+        const int n = __popc(moving);
 #pragma unroll
-        for (int b = 0; b < W; ++b)
-            if (dst[b]) *dst[b] = held[b];
+        for (int k = 0; k < W; ++k) {
+            const int b = moving ? __ffs(moving) - 1 : 0;
+            moving &= moving - 1;
+            char* at = base + head * (pages * page_bytes) + begin;
+            from_page[k] = (const V*)(at + __shfl_sync(0xffffffffu, src, b) * page_bytes), to_page[k] = (V*)(at + __shfl_sync(0xffffffffu, dst, b) * page_bytes);
+            f_of[k] = __shfl_sync(0xffffffffu, f, b), e_of[k] = k < n ? __shfl_sync(0xffffffffu, e, b) : 0;
+        }
+        const int vecs = (int)((end - begin) / (int)sizeof(V));
+        for (int i0 = lane; i0 < vecs; i0 += 32 * U) {
+            V held[U][W];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    const int i = i0 + 32 * u, at = i * (int)sizeof(V);
+                    if (k < n && at >= f_of[k] && at < e_of[k]) held[u][k] = from_page[k][i];
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    const int i = i0 + 32 * u, at = i * (int)sizeof(V);
+                    if (k < n && at >= f_of[k] && at < e_of[k]) to_page[k][i] = held[u][k];
+                }
+        }
     }
 }
 
@@ -104,14 +131,20 @@ template <typename V>
 void launch_pages(const PageTensors& t, int n, int groups, int width, int blocks_x, const int* table, int blocks, int page_size, const int* parents, const int* first,
                   const int* lengths, cudaStream_t st) {
     const dim3 grid(blocks_x, n, groups);
-    if (width <= 8) q6k_launch(reorder_pages_kernel<V, 8>, grid, RE_THREADS, 0, st, t, table, blocks, page_size, parents, first, lengths, width);
-    else q6k_launch(reorder_pages_kernel<V, RE_MAX_WIDTH>, grid, RE_THREADS, 0, st, t, table, blocks, page_size, parents, first, lengths, width);
+#define GO(W_, U_) q6k_launch(reorder_pages_kernel<V, W_, U_>, grid, RE_THREADS, 0, st, t, table, blocks, page_size, parents, first, lengths, width)
+    if (width <= 4) GO(4, 2);
+    else if (width <= 8) GO(8, 1);
+    else if (width <= 16) GO(16, 1);
+    else GO(RE_MAX_WIDTH, 1);
+#undef GO
 }
 
 template <typename V>
 void launch_slots(const SlotTensors& t, int n, int groups, int width, int blocks_x, const int* slots, const int* parents, cudaStream_t st) {
     const dim3 grid(blocks_x, n, groups);
-    if (width <= 8) q6k_launch(reorder_slots_kernel<V, 8>, grid, RE_THREADS, 0, st, t, slots, parents, width);
+    if (width <= 4) q6k_launch(reorder_slots_kernel<V, 4>, grid, RE_THREADS, 0, st, t, slots, parents, width);
+    else if (width <= 8) q6k_launch(reorder_slots_kernel<V, 8>, grid, RE_THREADS, 0, st, t, slots, parents, width);
+    else if (width <= 16) q6k_launch(reorder_slots_kernel<V, 16>, grid, RE_THREADS, 0, st, t, slots, parents, width);
     else q6k_launch(reorder_slots_kernel<V, RE_MAX_WIDTH>, grid, RE_THREADS, 0, st, t, slots, parents, width);
 }
 
@@ -134,12 +167,14 @@ Q6K_API int q6k_reorder_pages(int n, const long long* bases, const int* heads, c
         Q6K_REQUIRE(heads[i] > 0 && pages[i] > 0 && row_bytes[i] > 0, "reorder_pages: tensor %d has %d heads, %d pages, rows of %d bytes", i, heads[i], pages[i], row_bytes[i]);
         t.base[i] = (char*)bases[i], t.heads[i] = heads[i], t.pages[i] = pages[i], t.row_bytes[i] = row_bytes[i];
         all |= (unsigned long long)bases[i] | (unsigned long long)row_bytes[i];
-        const long long bytes = (long long)heads[i] * row_bytes[i];
-        if (bytes > most) most = bytes;
+        const long long pieces = (long long)blocks * heads[i] * (((long long)page_size * row_bytes[i] + RE_PIECE - 1) / RE_PIECE);
+        if (pieces > most) most = pieces;
     }
     const int vb = vector_bytes(all);
-    // enough blocks for every position of the table, at most eight rounds of the GPU's
-    const long long places = (long long)blocks * page_size * (most / vb), want = (places + RE_THREADS - 1) / RE_THREADS, cap = (148 * 8 * 8 + (long long)n * groups - 1) / ((long long)n * groups);
+    // Enough blocks for every piece of the table, and no more than some eight to an SM in all (three run at a time): how many positions move is known on
+    // the device only, and a block without any costs its start (48 tensors, eight requests of four beams, 21 positions of 1,789: 12.7 us with sixteen, 9.7
+    // with eight, 7.8 with four; but all of 4,096 positions of two requests: 197, 199 and 214 us).
+    const long long want = (most + RE_THREADS / 32 - 1) / (RE_THREADS / 32), cap = (148 * 8 + (long long)n * groups - 1) / ((long long)n * groups);
     const int bx = (int)(want < cap ? want : cap);
     if (vb == 16) launch_pages<uint4>(t, n, groups, width, bx, table, blocks, page_size, parents, first, lengths, st);
     else if (vb == 4) launch_pages<uint32_t>(t, n, groups, width, bx, table, blocks, page_size, parents, first, lengths, st);

@@ -2168,7 +2168,7 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Opti
 
 
 # --------------------------------------------------------------------------- beam search
-BEAM_MAX_WIDTH, BEAM_MAX_COUNT = 32, 256
+BEAM_MAX_WIDTH, BEAM_MAX_COUNT = 32, 128
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int):
