@@ -15,14 +15,15 @@ struct I8Args {
     void* out;
     long long lda, ldo;
     int rows, N, K, groups, pair_div;
+    int early;                     // the kernel before this one on the stream made a and a_scale and nothing else that is read here
     int epilogue, act;
     float act_param;
 };
 
 #define I8_OPERANDS                                                                                                                   \
     const void *a, long long lda, const float *a_scale, int rows, const void *w, const float *w_scale, const void *w2, const float *w2_scale, int N, int K, \
-        const int *a_rows, const int *offsets, int groups, const int *pair_expert, int pair_div, void *out, long long ldo, int epilogue, float act_param
-#define I8_NAMES a, lda, a_scale, rows, w, w_scale, w2, w2_scale, N, K, a_rows, offsets, groups, pair_expert, pair_div, out, ldo, epilogue, act_param
+        const int *a_rows, const int *offsets, int groups, const int *pair_expert, int pair_div, void *out, long long ldo, int epilogue, float act_param, int early
+#define I8_NAMES a, lda, a_scale, rows, w, w_scale, w2, w2_scale, N, K, a_rows, offsets, groups, pair_expert, pair_div, out, ldo, epilogue, act_param, early
 
 inline int i8_args(I8Args* p, const char* who, I8_OPERANDS) {
     const int act = epilogue >> 8, epi = epilogue & 255;         // the activation's code (q6k_activation) rides above bit 8
@@ -32,9 +33,13 @@ inline int i8_args(I8Args* p, const char* who, I8_OPERANDS) {
     Q6K_REQUIRE(act >= 0 && act <= (epi == I8_GATED ? Q6K_ACT_CLAMPED : 2), "%s: unknown activation %d", who, act);
     Q6K_REQUIRE(!(offsets && pair_expert) && groups >= 1 && pair_div >= 1, "%s: groups %d, pair_div %d", who, groups, pair_div);
     *p = I8Args{(const int8_t*)a, (const int8_t*)w, (const int8_t*)w2, a_scale, w_scale, w2_scale, a_rows, offsets, pair_expert, out, lda, ldo,
-                rows, N, K, groups, pair_div, epi, act, act_param};
+                rows, N, K, groups, pair_div, early, epi, act, act_param};
     return 0;
 }
+
+// Whether the launch may start while the kernel before it still runs (it then fetches weights before its wait).  Where the caller cannot say what that
+// kernel writes, it may be these very weights, just taken to 8 bits.
+inline bool i8_overlaps(const I8Args& p) { return p.early != 0 && q6k_pdl_mode() != 0; }
 
 // silu(g) u by a fast quotient: it is off by some 2^-21 of the value, and the result is rounded to bfloat16 (2^-8); where e^-g is beyond 2^126 the value
 // is below 1e-36 and comes out as zero.

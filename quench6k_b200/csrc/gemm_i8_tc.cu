@@ -117,7 +117,7 @@ __host__ __device__ constexpr int epilogue_warps(int bt) { return bt >= 64 ? 8 :
 template <int BT, int CTAS, bool DUAL>
 __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
                                                                                     const __grid_constant__ CUtensorMap tm_a, const TcArgs a) {
-    pdl_enter();
+    if (a.p.offsets) pdl_wait();
     constexpr int EW = epilogue_warps(BT), SPAN = BT / (EW / 4);       // rows that an epilogue warp takes of a tile
     constexpr uint32_t W_BYTES = WM * BK, A_BYTES = BT / CTAS * BK, STAGE_BYTES = W_BYTES + A_BYTES;
     constexpr int COLS = DUAL ? WM / 2 : WM;                           // output columns of a CTA's tile
@@ -172,11 +172,23 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     if constexpr (CTAS == 2) cluster_sync();             // both CTAs' barriers exist before either signals the other
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    pdl_launch();                                        // this block holds its tensor memory: a successor may come
     const int total = a.n_x * (p.offsets ? starts[p.groups] : a.n_y), kbs = (p.K + BK - 1) / BK;
 
     if (warp == 0) {
         if (elect_one()) {
             const uint64_t once = l2_evict_first_policy();
+            auto load_w = [&](uint32_t st, uint32_t fb, int i, int wy) {
+                if (rank == 0) mbar_expect_tx(fb, CTAS * STAGE_BYTES);
+                load<CTAS>(st, &tm_w, i * BK, wy, fb, a.w_once, once);
+                if (DUAL) load<CTAS>(st + W_BYTES / 2, &tm_w2, i * BK, wy, fb, a.w_once, once);
+            };
+            int pre = 0;                                 // k-blocks whose weights went out before the wait
+            for (int t = unit; t < total && pre < stages; t += units) {
+                const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
+                for (int i = 0; i < kbs && pre < stages; ++i, ++pre) load_w(ring + pre * STAGE_BYTES, full0 + 8 * pre, i, tl.g * p.N + tl.n0 + rank * COLS);
+            }
+            pdl_wait();
             int s = 0;
             uint32_t st = ring, phase = 0;
             bool ok = true;
@@ -185,14 +197,16 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
                 const int wy = tl.g * p.N + tl.n0 + rank * COLS, ay = tl.row0 + rank * (BT / CTAS);
                 for (int i = 0; i < kbs; ++i) {
                     const uint32_t fb = full0 + 8 * s;
-                    if (!mbar_wait(empty0 + 8 * s, phase ^ 1)) {
-                        atomicExch(&g_i8_status, 21);
-                        ok = false;
-                        break;
+                    if (pre > 0) {                       // a fresh stage, its weights on the way
+                        --pre;
+                    } else {
+                        if (!mbar_wait(empty0 + 8 * s, phase ^ 1)) {
+                            atomicExch(&g_i8_status, 21);
+                            ok = false;
+                            break;
+                        }
+                        load_w(st, fb, i, wy);
                     }
-                    if (rank == 0) mbar_expect_tx(fb, CTAS * STAGE_BYTES);
-                    load<CTAS>(st, &tm_w, i * BK, wy, fb, a.w_once, once);
-                    if (DUAL) load<CTAS>(st + W_BYTES / 2, &tm_w2, i * BK, wy, fb, a.w_once, once);
                     load<CTAS>(st + W_BYTES, &tm_a, i * BK, ay, fb, false, once);
                     if (++s == stages) s = 0, st = ring, phase ^= 1;
                     else st += STAGE_BYTES;
@@ -235,6 +249,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
         const uint32_t mine = swap0 + (warp - 2) * SWAP_BYTES, theirs = swap0 + ((part << 2 | ((quarter ^ 2) + 2 & 3)) * SWAP_BYTES);
         int nt = 0, turn = 0;
         bool ok = true;
+        pdl_wait();                                      // the rows' scales come from the kernel before, and the output may still be in use by it
         for (int t = unit; t < total; t += units, ++nt) {
             const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
             const int buf = nt & 1, n = tl.n0 + rank * COLS + (DUAL ? quarter & 1 : quarter) * 32 + lane;
@@ -419,12 +434,42 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
     const int units = sm_count() / CTAS;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS * (unsigned)(total < units ? total : units)), cfg.blockDim = dim3(64 + 32 * EW), cfg.dynamicSmemBytes = smem, cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr, cfg.numAttrs = CTAS == 2 ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    if (CTAS == 2) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = CTAS, attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (i8_overlaps(p)) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    cfg.attrs = attr;
     cudaLaunchKernelEx(&cfg, gemm_i8_tc_kernel<BT, CTAS, DUAL>, tw, tw2, ta, t);
     return q6k_check_launch("gemm_i8");
+}
+
+// Rows of a tile (negative: a pair of CTAs).  A unit's time for one tile of K = 2,048, in tenths of a microsecond, measured over many tiles (8,192 x 2
+// columns): a wide tile re-reads less and feeds the tensor cores better, a narrow one leaves fewer units idle in the last round.  With the least
+// rounds x time, 1,522 rows x (2 x 8,192), K 2,048 take 41.1 us on pairs of 192 (42.2 of 256; 53.7 with single CTAs of 128), 256 rows x 2,048 take
+// 6.6 us on tiles of 32 (7.2 of 128, 11.1 on pairs), 64 rows x (2 x 8,192) 9.7 on 64 (12.8 on 32), all in a graph with weights from HBM.
+// Grouped rows: the experts' shares are known on the device only, so half as much again as an even share.
+int choose_tile(const I8Args& p, bool dual) {
+    if (p.offsets) {
+        const int share = p.rows / p.groups + p.rows / p.groups / 2;
+        return share <= 32 ? 32 : share <= 64 ? 64 : 128;
+    }
+    static const int tiles[][2] = {{32, 35}, {64, 38}, {128, 47}, {256, 76}, {-192, 52}, {-256, 69}};
+    long long best = -1;
+    int pick = 0;
+    for (auto& t : tiles) {
+        const int bt = t[0] < 0 ? -t[0] : t[0], ctas = t[0] < 0 ? 2 : 1, cols = ctas * (dual ? WM / 2 : WM);
+        const long long units = sm_count() / ctas, count = (long long)((p.N + cols - 1) / cols) * ((p.rows + bt - 1) / bt);
+        const long long cost = (count + units - 1) / units * t[1];
+        if (best < 0 || cost < best) best = cost, pick = t[0];
+    }
+    return pick;
 }
 
 }  // namespace
@@ -443,7 +488,7 @@ Q6K_API int q6k_gemm_i8_tc(I8_OPERANDS, int a_total, int tile, cudaStream_t st) 
     if (rows == 0) return 0;
     Q6K_REQUIRE(!pair_expert && groups <= MAX_GROUPS && (long long)groups * N < (1LL << 31) - 256 && a_total >= rows, "gemm_i8: %d groups of %d columns, %d rows of %d", groups, N, rows, a_total);
     const bool dual = w2 != nullptr;
-    if (tile == 0) tile = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    if (tile == 0) tile = choose_tile(t.p, dual);
 #define GO(T_, BT_, CTAS_) \
     case T_: return dual ? launch<BT_, CTAS_, true>(t, a_total, st) : launch<BT_, CTAS_, false>(t, a_total, st)
     switch (tile) {

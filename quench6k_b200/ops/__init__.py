@@ -2104,13 +2104,15 @@ _i8_tile = 0
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
             accumulate: bool = False, w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None,
-            offsets: Optional[torch.Tensor] = None, a_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+            offsets: Optional[torch.Tensor] = None, a_rows: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
     """y[r, n] = a_scale[r] * w_scale[n] * sum_k a[r, k] w[n, k] of int8 operands, the sum exact in 32-bit integers.
 
     a: int8 [*, K], a_scale: float32 [*]; w: int8 [N, K] with w_scale float32 [N].  Stored in float32, or added into `out`
     (accumulate).  With w2 the gated epilogue act(y) * y2 (act None: silu), with act alone act(y); both leave in bfloat16.
     a_rows (int32 [rows]): row r of the product is row a_rows[r] of a.  offsets (int32 [G + 1], ascending from 0) with w [G, N, K]
-    and w_scale [G, N]: rows offsets[g] .. offsets[g + 1] - 1 go against matrix g; rows behind the last offset are left as they were."""
+    and w_scale [G, N]: rows offsets[g] .. offsets[g + 1] - 1 go against matrix g; rows behind the last offset are left as they were.
+    early: the caller's word that the kernel before this call made a and a_scale and nothing else that is read here: the weights
+    are then fetched while it ends."""
     _need_rows(a, "a")
     if a.dtype != torch.int8:
         raise KernelError(f"a has dtype {a.dtype}, expected torch.int8")
@@ -2132,14 +2134,14 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     lda = a.stride(0) if total > 1 else K
     if rows <= 16 and not grouped:
         _call("q6k_gemm_i8_rows", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-              _ptr(a_rows), _ptr(None), _i(1), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _stream())
+              _ptr(a_rows), _ptr(None), _i(1), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(early), _stream())
         return out
     if a_rows is not None:
         if not a.is_contiguous():
             raise KernelError("gemm_i8: rows that are picked lie side by side")
         a, total, lda = gather_rows(a, a_rows), rows, K
     _call("q6k_gemm_i8_tc", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(total), _i(_i8_tile), _stream())
+          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(early), _i(total), _i(_i8_tile), _stream())
     return out
 
 
@@ -2151,7 +2153,7 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Opti
     pair_expert[y]; a pair that names no matrix is left as it was."""
     q, scale = quantize_rows(x)
     if pair_expert is None:
-        return gemm_i8(q, scale, w, w_scale, out=out, accumulate=accumulate, w2=w2, w2_scale=w2_scale, act=act)
+        return gemm_i8(q, scale, w, w_scale, out=out, accumulate=accumulate, w2=w2, w2_scale=w2_scale, act=act, early=True)
     T, K = x.shape
     groups, N = _i8_weights(w, w_scale, w2, w2_scale, K, True, "linear_i8")
     _need(pair_expert, "pair_expert", torch.int32)
@@ -2163,7 +2165,7 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Opti
         raise KernelError("linear_i8: a gated product is stored, not added")
     out = _i8_out(out, pairs, N, epi, x.device, "linear_i8")
     _call("q6k_gemm_i8_rows", _ptr(q), _ll(K), _ptr(scale), _i(pairs), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-          _ptr(None), _ptr(None), _i(groups), _ptr(pair_expert), _i(pair_div), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _stream())
+          _ptr(None), _ptr(None), _i(groups), _ptr(pair_expert), _i(pair_div), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(1), _stream())
     return out
 
 
