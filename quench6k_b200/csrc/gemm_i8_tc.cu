@@ -36,7 +36,7 @@ struct TcArgs {
 };
 
 // D: 32-bit integers, A and B signed 8-bit integers, both K-major, M rows, N = n.
-__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+__device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 template <int CTAS>
@@ -86,13 +86,15 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Which weights, which rows.
+// Which weights, which rows; n: the rows that are loaded and multiplied, the tile's rows rounded up.  (With whole tiles throughout, 16,384 rows of 256 experts,
+// 2 x 512 columns, K 2,048, took 106 us; the L2 cache delivered 12 TB/s, a good third of it for rows of other experts.)
 struct Tile {
-    int g, n0, row0, row_end;
+    int g, n0, row0, row_end, n;
 };
 
-// Tile t: tiles along N fastest (units side by side share the rows).  starts (grouped): how many row tiles come before each group.
-template <int BT>
+// Tile t: tiles along N fastest (units side by side share the rows).  Grouped: starts[g], in shared memory, is how many row tiles come before group g, and
+// behind the groups + 1 of them lie the groups' first rows.
+template <int BT, int CTAS>
 __device__ __forceinline__ Tile tile_of(const TcArgs& a, int t, int cols, const int* starts) {
     Tile o;
     const int y = t / a.n_x;
@@ -105,10 +107,12 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, int t, int cols, const 
             else hi = mid - 1;
         }
         o.g = lo;
-        o.row0 = a.p.offsets[lo] + (y - starts[lo]) * BT, o.row_end = min(a.p.offsets[lo + 1], a.p.rows);
+        const int* offsets = starts + a.p.groups + 1;
+        o.row0 = offsets[lo] + (y - starts[lo]) * BT, o.row_end = offsets[lo + 1];
     } else {
         o.g = 0, o.row0 = y * BT, o.row_end = a.p.rows;
     }
+    o.n = min(BT, (o.row_end - o.row0 + 32 * CTAS - 1) / (32 * CTAS) * (32 * CTAS));
     return o;
 }
 
@@ -116,9 +120,10 @@ __host__ __device__ constexpr int epilogue_warps(int bt) { return bt >= 64 ? 8 :
 
 template <int BT, int CTAS, bool DUAL>
 __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
-                                                                                    const __grid_constant__ CUtensorMap tm_a, const TcArgs a) {
-    if (a.p.offsets) pdl_wait();
-    constexpr int EW = epilogue_warps(BT), SPAN = BT / (EW / 4);       // rows that an epilogue warp takes of a tile
+                                                                                    const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
+                                                                                    const TcArgs a) {
+    if (a.p.offsets && !a.p.early) pdl_wait();
+    constexpr int EW = epilogue_warps(BT), SPAN = BT / (EW / 4);       // rows that an epilogue warp takes of a whole tile
     constexpr uint32_t W_BYTES = WM * BK, A_BYTES = BT / CTAS * BK, STAGE_BYTES = W_BYTES + A_BYTES;
     constexpr int COLS = DUAL ? WM / 2 : WM;                           // output columns of a CTA's tile
     constexpr uint32_t TMEM_COLS = 2 * BT <= 32 ? 32 : 2 * BT <= 64 ? 64 : 2 * BT <= 128 ? 128 : 2 * BT <= 256 ? 256 : 512;
@@ -151,20 +156,26 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
-    } else if (warp == 2 && p.offsets) {                 // row tiles before each group
-        int before = 0;
-        for (int g0 = 0; g0 <= p.groups; g0 += 32) {
-            const int g = g0 + lane;
-            const int rows = g < p.groups ? min(p.offsets[g + 1], p.rows) - p.offsets[g] : 0;
-            const int mine = rows > 0 ? (rows + BT - 1) / BT : 0;
-            int upto = mine;
+    }
+    if (p.offsets) {                                     // row tiles before each group (everyone fetches, so that one latency passes and not one for each 32 groups)
+        int* offsets = starts + p.groups + 1;
+        for (int g = threadIdx.x; g <= p.groups; g += blockDim.x) offsets[g] = min(max(p.offsets[g], 0), p.rows);
+        __syncthreads();
+        if (warp == 2) {
+            int before = 0;
+            for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+                const int g = g0 + lane;
+                const int rows = g < p.groups ? offsets[g + 1] - offsets[g] : 0;
+                const int mine = rows > 0 ? (rows + BT - 1) / BT : 0;
+                int upto = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                if (g <= p.groups) starts[g] = before + upto - mine;
+                before += __shfl_sync(0xffffffffu, upto, 31);
             }
-            if (g <= p.groups) starts[g] = before + upto - mine;
-            before += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
     tc_fence_before();
@@ -178,23 +189,23 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     if (warp == 0) {
         if (elect_one()) {
             const uint64_t once = l2_evict_first_policy();
-            auto load_w = [&](uint32_t st, uint32_t fb, int i, int wy) {
-                if (rank == 0) mbar_expect_tx(fb, CTAS * STAGE_BYTES);
+            auto load_w = [&](uint32_t st, uint32_t fb, int i, int wy, int n) {
+                if (rank == 0) mbar_expect_tx(fb, CTAS * W_BYTES + n * BK);
                 load<CTAS>(st, &tm_w, i * BK, wy, fb, a.w_once, once);
                 if (DUAL) load<CTAS>(st + W_BYTES / 2, &tm_w2, i * BK, wy, fb, a.w_once, once);
             };
-            int pre = 0;                                 // k-blocks whose weights went out before the wait
-            for (int t = unit; t < total && pre < stages; t += units) {
-                const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
-                for (int i = 0; i < kbs && pre < stages; ++i, ++pre) load_w(ring + pre * STAGE_BYTES, full0 + 8 * pre, i, tl.g * p.N + tl.n0 + rank * COLS);
+            int pre = 0;                                 // k-blocks whose weights went out before the wait (with nothing to wait for, the first rows would queue behind them)
+            for (int t = unit; p.early && t < total && pre < stages; t += units) {
+                const Tile tl = tile_of<BT, CTAS>(a, t, CTAS * COLS, starts);
+                for (int i = 0; i < kbs && pre < stages; ++i, ++pre) load_w(ring + pre * STAGE_BYTES, full0 + 8 * pre, i, tl.g * p.N + tl.n0 + rank * COLS, tl.n);
             }
             pdl_wait();
             int s = 0;
             uint32_t st = ring, phase = 0;
             bool ok = true;
             for (int t = unit; t < total && ok; t += units) {
-                const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
-                const int wy = tl.g * p.N + tl.n0 + rank * COLS, ay = tl.row0 + rank * (BT / CTAS);
+                const Tile tl = tile_of<BT, CTAS>(a, t, CTAS * COLS, starts);
+                const int wy = tl.g * p.N + tl.n0 + rank * COLS, ay = tl.row0 + rank * (tl.n / CTAS);
                 for (int i = 0; i < kbs; ++i) {
                     const uint32_t fb = full0 + 8 * s;
                     if (pre > 0) {                       // a fresh stage, its weights on the way
@@ -205,9 +216,11 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
                             ok = false;
                             break;
                         }
-                        load_w(st, fb, i, wy);
+                        load_w(st, fb, i, wy, tl.n);
                     }
-                    load<CTAS>(st + W_BYTES, &tm_a, i * BK, ay, fb, false, once);
+                    if (tl.n == BT) load<CTAS>(st + W_BYTES, &tm_a, i * BK, ay, fb, false, once);
+                    else
+                        for (int c = 0; c < tl.n / CTAS; c += 32) load<CTAS>(st + W_BYTES + c * BK, &tm_a32, i * BK, ay + c, fb, false, once);
                     if (++s == stages) s = 0, st = ring, phase ^= 1;
                     else st += STAGE_BYTES;
                 }
@@ -215,7 +228,6 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
         }
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
-            constexpr uint32_t idesc = idesc_i8(CTAS * WM, BT);
             int s = 0, nt = 0;
             uint32_t st = ring, phase = 0;
             bool ok = true;
@@ -226,6 +238,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
                     break;
                 }
                 tc_fence_after();
+                const uint32_t idesc = idesc_i8(CTAS * WM, tile_of<BT, CTAS>(a, t, CTAS * COLS, starts).n);
                 for (int i = 0; i < kbs; ++i) {
                     if (!mbar_wait(full0 + 8 * s, phase)) {
                         atomicExch(&g_i8_status, 22);
@@ -251,19 +264,20 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
         bool ok = true;
         pdl_wait();                                      // the rows' scales come from the kernel before, and the output may still be in use by it
         for (int t = unit; t < total; t += units, ++nt) {
-            const Tile tl = tile_of<BT>(a, t, CTAS * COLS, starts);
+            const Tile tl = tile_of<BT, CTAS>(a, t, CTAS * COLS, starts);
             const int buf = nt & 1, n = tl.n0 + rank * COLS + (DUAL ? quarter & 1 : quarter) * 32 + lane;
             const long long at_n = (long long)tl.g * p.N + n;
             const float ws = n < p.N ? p.w_scale[at_n] : 0.0f, ws2 = DUAL && n < p.N ? p.w2_scale[at_n] : 0.0f;
-            const int end = min(SPAN, tl.row_end - tl.row0 - part * SPAN), row0 = tl.row0 + part * SPAN;
+            const int span = tl.n == BT ? SPAN : (tl.n / (EW / 4) + 31) / 32 * 32, row0 = tl.row0 + part * span;      // this warp's rows of the tile
+            const int end = min(span, tl.row_end - row0);
             // the rows' scales go to shared memory while the accumulator fills (read from global memory where they are needed, every 16 rows waited for them:
             // 2,048 x 2,048 x 2,048 16.0 us, 12.1 now)
             const uint32_t scales = scales0 + (warp - 2) * SCALE_BYTES;
             __syncwarp();
 #pragma unroll
-            for (int c = 0; c < SPAN; c += 32) {
+            for (int c = 0; c < SPAN; c += 32) {             // (span is at most SPAN)
                 const int r = row0 + c + lane;
-                const float xs = r < tl.row_end ? p.a_scale[p.a_rows ? p.a_rows[r] : r] : 0.0f;
+                const float xs = r < tl.row_end ? p.a_scale[r] : 0.0f;
                 asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + (c + lane) * 4), "f"(xs) : "memory");
             }
             __syncwarp();
@@ -277,7 +291,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
                 ok = false;                              // on to the barriers that a partner may be waiting at, with no further wait
             }
             tc_fence_after();
-            const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BT + part * SPAN;
+            const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BT + part * span;
             auto release = [&] {
                 tc_fence_before();
                 __syncwarp();
@@ -381,6 +395,26 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     }
 }
 
+// Rows picked from a with their scales, a warp each, so that the tiles' loads find them side by side.
+__global__ void __launch_bounds__(256) gather_i8_kernel(const int8_t* a, long long lda, const float* a_scale, const int* a_rows, int rows, int K, int8_t* out, float* scale) {
+    pdl_enter();
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= rows) return;
+    const int from = a_rows[r];
+    const int8_t* src = a + from * lda;
+    int8_t* dst = out + (long long)r * K;
+    if (lane == 0) scale[r] = a_scale[from];
+    for (int k0 = lane * 16; k0 < K; k0 += 4 * 512) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (k0 + i * 512 < K) v[i] = *(const uint4*)(src + k0 + i * 512);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (k0 + i * 512 < K) *(uint4*)(dst + k0 + i * 512) = v[i];
+    }
+}
+
 // ---------------------------------------------------------------------------------------- host
 // An int8 matrix [rows, cols] in boxes of [box_rows, 128] with the 128-byte swizzle; reads outside give zeros.
 int make_i8_map(CUtensorMap* map, const void* base, long long rows, int cols, long long pitch, int box_rows, bool weights) {
@@ -410,14 +444,15 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
     const I8Args& p = t.p;
     constexpr int EW = epilogue_warps(BT), COLS = CTAS * (DUAL ? WM / 2 : WM);
     constexpr int stage = WM * BK + BT / CTAS * BK;
-    CUtensorMap tw, tw2, ta;
+    CUtensorMap tw, tw2, ta, ta32;
     const int w_box = DUAL ? WM / 2 : WM;
     if (int rc = make_i8_map(&tw, p.w, (long long)p.groups * p.N, p.K, p.K, w_box, true)) return rc;
     tw2 = tw;
     if (DUAL)
         if (int rc = make_i8_map(&tw2, p.w2, (long long)p.groups * p.N, p.K, p.K, w_box, true)) return rc;
     if (int rc = make_i8_map(&ta, p.a, a_total, p.K, p.lda, BT / CTAS, false)) return rc;
-    const int extra = (DUAL ? EW * SWAP_BYTES : 0) + EW * SCALE_BYTES + (p.offsets ? (p.groups + 1) * 4 : 0);
+    if (int rc = make_i8_map(&ta32, p.a, a_total, p.K, p.lda, 32, false)) return rc;
+    const int extra = (DUAL ? EW * SWAP_BYTES : 0) + EW * SCALE_BYTES + (p.offsets ? 2 * (p.groups + 1) * 4 : 0);
     t.stages = (222 * 1024 - extra) / stage;
     if (t.stages > MAX_STAGES) t.stages = MAX_STAGES;
     t.n_x = (p.N + COLS - 1) / COLS, t.n_y = (p.rows + BT - 1) / BT;
@@ -446,7 +481,7 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
         ++cfg.numAttrs;
     }
     cfg.attrs = attr;
-    cudaLaunchKernelEx(&cfg, gemm_i8_tc_kernel<BT, CTAS, DUAL>, tw, tw2, ta, t);
+    cudaLaunchKernelEx(&cfg, gemm_i8_tc_kernel<BT, CTAS, DUAL>, tw, tw2, ta, ta32, t);
     return q6k_check_launch("gemm_i8");
 }
 
@@ -480,13 +515,21 @@ Q6K_API int q6k_gemm_i8_status() {
     return v;
 }
 
-// See ops.gemm_i8 for the operands.  a_rows: the rows of a have been gathered already, the list is for their scales; a has `a_total` rows.
-// tile: rows of a tile (0: chosen here), negative for pairs of CTAs.
-Q6K_API int q6k_gemm_i8_tc(I8_OPERANDS, int a_total, int tile, cudaStream_t st) {
+// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered, gathered_scale (with a_rows): int8 [rows, K] and FP32 [rows] of scratch.
+// tile: rows of a tile, negative for pairs of CTAs (0: chosen here).
+Q6K_API int q6k_gemm_i8_tc(I8_OPERANDS, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st) {
     TcArgs t;
     if (int rc = i8_args(&t.p, "gemm_i8", I8_NAMES)) return rc;
     if (rows == 0) return 0;
-    Q6K_REQUIRE(!pair_expert && groups <= MAX_GROUPS && (long long)groups * N < (1LL << 31) - 256 && a_total >= rows, "gemm_i8: %d groups of %d columns, %d rows of %d", groups, N, rows, a_total);
+    Q6K_REQUIRE(!pair_expert && groups <= MAX_GROUPS && (long long)groups * N < (1LL << 31) - 256, "gemm_i8: %d groups (at most %d) of %d columns", groups, MAX_GROUPS, N);
+    if (a_rows) {
+        Q6K_REQUIRE(gathered && gathered_scale && ((uintptr_t)gathered & 15) == 0, "gemm_i8: no scratch for the rows that are picked");
+        q6k_launch(gather_i8_kernel, (rows + 7) / 8, 256, 0, st, t.p.a, lda, a_scale, a_rows, rows, K, (int8_t*)gathered, gathered_scale);
+        if (int rc = q6k_check_launch("gemm_i8: gather")) return rc;
+        t.p.a = (const int8_t*)gathered, t.p.a_scale = gathered_scale, t.p.a_rows = nullptr, t.p.lda = K, t.p.early = 1;
+        a_total = rows;
+    }
+    Q6K_REQUIRE(a_total >= rows, "gemm_i8: %d rows of %d", rows, a_total);
     const bool dual = w2 != nullptr;
     if (tile == 0) tile = choose_tile(t.p, dual);
 #define GO(T_, BT_, CTAS_) \

@@ -2136,12 +2136,12 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
         _call("q6k_gemm_i8_rows", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
               _ptr(a_rows), _ptr(None), _i(1), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(early), _stream())
         return out
+    gathered = gathered_scale = None
     if a_rows is not None:
-        if not a.is_contiguous():
-            raise KernelError("gemm_i8: rows that are picked lie side by side")
-        a, total, lda = gather_rows(a, a_rows), rows, K
+        gathered, gathered_scale = torch.empty((rows, K), dtype=torch.int8, device=a.device), torch.empty(rows, dtype=torch.float32, device=a.device)
     _call("q6k_gemm_i8_tc", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(early), _i(total), _i(_i8_tile), _stream())
+          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(early), _i(total), _ptr(gathered),
+          _ptr(gathered_scale), _i(_i8_tile), _stream(), launches=(rows > 0) * (1 if a_rows is None else 2))
     return out
 
 
