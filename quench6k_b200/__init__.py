@@ -9,5 +9,5 @@ from .models import sigusun as _sigusun   # noqa: F401  (registers Sigusun)
 from .models import kitodra as _kitodra   # noqa: F401  (registers Kitodra)
 from .models import gunenex as _gunenex   # noqa: F401  (registers Gunenex)
 from .models import kodatar as _kodatar   # noqa: F401  (registers Kodatar)
-from .sampling.params import SamplingParams      # noqa: F401
-from .engine.engine import Engine, RequestOutput   # noqa: F401
+from .sampling.params import BeamParams, SamplingParams      # noqa: F401
+from .engine.engine import BeamOutput, Engine, RequestOutput   # noqa: F401

@@ -23,7 +23,7 @@ def _generate(a) -> int:
     import torch
     from . import ops
     from .engine import Engine
-    from .sampling import SamplingParams
+    from .sampling import BeamParams, SamplingParams
 
     page = a.page_size
     if a.model:
@@ -32,14 +32,14 @@ def _generate(a) -> int:
         page = page or getattr(cfg, "kv_page_size", None) or 16
         num_pages = a.num_pages or (a.context + page - 1) // page
         eng = Engine.from_folder(a.model, dtype=a.dtype, page_size=page, num_pages=num_pages,
-                                 max_batch_tokens=a.max_batch_tokens)
+                                 max_batch_tokens=a.max_batch_tokens, weights=a.weights)
     else:
         from .config.registry import load_config
         _, cfg = load_config(a.random)
         page = page or getattr(cfg, "kv_page_size", None) or 16
         num_pages = a.num_pages or (a.context + page - 1) // page
         eng = Engine.from_random(cfg, seed=a.seed, dtype=a.dtype, page_size=page, num_pages=num_pages,
-                                 max_batch_tokens=a.max_batch_tokens)
+                                 max_batch_tokens=a.max_batch_tokens, weights=a.weights)
     vocab = eng.runner.vocab_size
     if a.prompt_ids:
         ids = [int(x) for x in a.prompt_ids.split(",") if x.strip()]
@@ -47,6 +47,15 @@ def _generate(a) -> int:
         g = torch.Generator().manual_seed(a.seed)
         ids = torch.randint(0, vocab, (a.prompt_len,), generator=g).tolist()
     print(f"prompt: {len(ids)} tokens")
+    if a.beams:
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        outs = eng.beam_search([ids], BeamParams(width=a.beams, max_tokens=a.n, length_penalty=a.length_penalty))[0]
+        took = time.perf_counter() - t0
+        for o in outs:
+            print(f"{o.score:.4f} (sum {o.logprob:.4f}, {o.finish_reason}) ids: {o.tokens}")
+        print(f"{a.beams} beams, {max((len(o.tokens) for o in outs), default=0)} tokens in {took:.3f}s")
+        return 0
     params = SamplingParams(max_tokens=a.n, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p,
                             seed=a.sample_seed)
     rid = eng.add_request(ids, params)
@@ -87,8 +96,8 @@ def _runner(a, tokens: int):
     page = a.page_size or getattr(cfg, "kv_page_size", None) or 16
     num_pages = (tokens + page - 1) // page + 1
     if a.model:
-        return ModelRunner.from_folder(a.model, dtype=a.dtype, page_size=page, num_pages=num_pages, max_requests=2)
-    return ModelRunner.from_random(cfg, a.seed, dtype=a.dtype, page_size=page, num_pages=num_pages, max_requests=2)
+        return ModelRunner.from_folder(a.model, dtype=a.dtype, page_size=page, num_pages=num_pages, max_requests=2, weights=a.weights)
+    return ModelRunner.from_random(cfg, a.seed, dtype=a.dtype, page_size=page, num_pages=num_pages, max_requests=2, weights=a.weights)
 
 
 def _corpus(path, need: int, vocab: int, seed: int):
@@ -239,6 +248,9 @@ def main(argv=None) -> int:
     g.add_argument("--min-p", type=float, default=0.0)
     g.add_argument("--sample-seed", type=int, default=0)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
+    g.add_argument("--weights", default=None, choices=["int8"], help="keep the large matrices in 8 bits")
+    g.add_argument("--beams", type=int, default=0, help="beam search with this many beams (--context counts the tokens of all of them) instead of sampling")
+    g.add_argument("--length-penalty", type=float, default=1.0)
     g.add_argument("--page-size", type=int, default=None)
     g.add_argument("--num-pages", type=int, default=None)
     g.add_argument("--max-batch-tokens", type=int, default=2048)
@@ -249,6 +261,7 @@ def main(argv=None) -> int:
         src.add_argument("--random", metavar="CONFIG.json", help="random weights from this configuration")
         q.add_argument("--seed", type=int, default=0, help="seed of the random weights (and of random token ids)")
         q.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
+        q.add_argument("--weights", default=None, choices=["int8"], help="keep the large matrices in 8 bits")
         q.add_argument("--page-size", type=int, default=None)
         q.add_argument("--max-batch-tokens", type=int, default=2048, help="tokens of a prompt portion")
 

@@ -5,7 +5,7 @@
 
 Token ids in, token ids out (the reference's tokenizer and chat template,
 crates/cli/src/chat.rs, are outside this engine).  `step()` runs one scheduled batch;
-`generate()` runs until every given prompt has finished.
+`generate()` runs until every given prompt has finished; `beam_search()` finds the best continuations of prompts.
 
 While no live request uses penalties, `step()` does not wait for the tokens of the step it has just
 launched: the choice (argmax, or the sampler's arithmetic on the candidate pools with a uniform the
@@ -27,9 +27,10 @@ from typing import Dict, Hashable, List, Optional, Sequence, Union
 import torch
 
 from .. import ops
-from ..sampling import Sampler, SamplingParams, SplitMix64
+from ..sampling import BeamParams, Sampler, SamplingParams, SplitMix64
 from ..sampling.sampler import ROW_RECORD, device_rows, pool_size
 from .batch import StepEntry
+from .beams import BeamOutput, BeamSearch
 from .runner import ModelRunner
 from .scheduler import FINISH_CANCELLED, Request, ScheduledStep, Scheduler
 
@@ -76,15 +77,16 @@ class Engine:
     @classmethod
     def from_folder(cls, folder: str, dtype="bfloat16", device="cuda:0", page_size: Optional[int] = None,
                     num_pages: Union[int, Sequence[int]] = 256, max_requests: int = 64, max_batch_tokens: int = 2048,
-                    tensor_cores: bool = True, lookahead: bool = True) -> "Engine":
-        runner = ModelRunner.from_folder(folder, dtype, device, page_size, num_pages, max_requests, tensor_cores)
+                    tensor_cores: bool = True, lookahead: bool = True, weights: Optional[str] = None) -> "Engine":
+        """weights: None, or "int8" to keep the large matrices in 8 bits (engine.runner.make_runtime says which)."""
+        runner = ModelRunner.from_folder(folder, dtype, device, page_size, num_pages, max_requests, tensor_cores, weights=weights)
         return cls(runner, max_batch_tokens, lookahead=lookahead)
 
     @classmethod
     def from_random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", page_size: Optional[int] = None,
                     num_pages: Union[int, Sequence[int]] = 256, max_requests: int = 64, max_batch_tokens: int = 2048,
-                    tensor_cores: bool = True, lookahead: bool = True) -> "Engine":
-        runner = ModelRunner.from_random(config, seed, dtype, device, page_size, num_pages, max_requests, tensor_cores)
+                    tensor_cores: bool = True, lookahead: bool = True, weights: Optional[str] = None) -> "Engine":
+        runner = ModelRunner.from_random(config, seed, dtype, device, page_size, num_pages, max_requests, tensor_cores, weights=weights)
         return cls(runner, max_batch_tokens, lookahead=lookahead)
 
     # ------------------------------------------------------------------ requests
@@ -248,3 +250,13 @@ class Engine:
             for out in self.step():
                 results[out.rid] = out
         return [results[r] for r in rids]
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], params: Optional[BeamParams] = None) -> List[List[BeamOutput]]:
+        """The best continuations of every prompt by beam search, best first, in the order of the prompts.  It has the runner to
+        itself: refused while requests are unfinished.  Raises OutOfPages or OutOfSlots where not even one prompt's beams fit."""
+        params = params or BeamParams()
+        if self.has_unfinished():
+            raise RuntimeError("beam search while requests are unfinished")
+        if not params.stop_tokens and self.eos:
+            params = BeamParams(**{**params.__dict__, "stop_tokens": list(self.eos)})
+        return BeamSearch(self.runner, self.scheduler.max_batch_tokens).run(prompts, params)

@@ -11,6 +11,7 @@ from __future__ import annotations
 from collections import OrderedDict
 from typing import Dict, Hashable, List, Optional, Sequence, Union
 
+import numpy as np
 import torch
 
 from .. import ops
@@ -29,6 +30,17 @@ def parse_dtype(d) -> torch.dtype:
     if d not in _DTYPES:
         raise ValueError(f"dtype {d!r} is neither bfloat16 nor float32")
     return _DTYPES[d]
+
+
+def make_runtime(device, dtype, tensor_cores: bool = True, weights: Optional[str] = None) -> Runtime:
+    """weights: None (the matrices in the operand dtype), or "int8" (bfloat16 only): the projections of attention, the dense and
+    routed feed-forwards and an untied LM head are kept in 8 bits with a scale for each output channel."""
+    if weights not in (None, "int8"):
+        raise ValueError(f"weights {weights!r}: None or 'int8'")
+    rt = Runtime(torch.device(device), parse_dtype(dtype), tensor_cores, weights == "int8")
+    if rt.int8_weights and rt.is_fp32:
+        raise ValueError("weights in 8 bits go with bfloat16: float32 is the path without any reduced precision")
+    return rt
 
 
 class ModelRunner:
@@ -97,6 +109,7 @@ class ModelRunner:
         # ids sampled on the device by the step before (greedy decoding that does not wait for the host)
         self.sampled = torch.zeros(max(64, max_requests), dtype=torch.int32, device=rt.device)
         self._feed_limit = 0
+        self._page_sets = self._slot_set = None            # the pools and the states as the reordering kernels take them, made at its first use
         self._pinned: Optional[torch.Tensor] = None
         self._pinned_free: Optional[torch.cuda.Event] = None      # set once the last upload has left the pinned block
 
@@ -104,10 +117,10 @@ class ModelRunner:
     @classmethod
     def from_folder(cls, folder: str, dtype="bfloat16", device="cuda:0", page_size: Optional[int] = None,
                     num_pages: Union[int, Sequence[int]] = 256, max_requests: int = 64, tensor_cores: bool = True,
-                    cuda_graphs: bool = True):
+                    cuda_graphs: bool = True, weights: Optional[str] = None):
+        rt = make_runtime(device, dtype, tensor_cores, weights)
         arch, cfg = load_config(folder)
         model = DecoderModel(arch.build_spec(cfg))
-        rt = Runtime(torch.device(device), parse_dtype(dtype), tensor_cores)
         get = load_folder(folder, model.tensors(), model.spec.name_alias, device=rt.device, ignorable=model.spec.ignorable)
         model.bind(get, rt)
         if get.uploader is not None:
@@ -118,13 +131,13 @@ class ModelRunner:
     @classmethod
     def from_random(cls, cfg, seed: int, dtype="bfloat16", device="cuda:0", page_size: Optional[int] = None,
                     num_pages: Union[int, Sequence[int]] = 256, max_requests: int = 64, tensor_cores: bool = True,
-                    arch=None, cuda_graphs: bool = True):
+                    arch=None, cuda_graphs: bool = True, weights: Optional[str] = None):
         """Random weights made on the device from the typed config and a seed (no files)."""
         from ..config.registry import get_architecture
         arch = arch or get_architecture(cfg.architectures[0])
         spec = arch.build_spec(cfg)
         model = DecoderModel(spec)
-        rt = Runtime(torch.device(device), parse_dtype(dtype), tensor_cores)
+        rt = make_runtime(device, dtype, tensor_cores, weights)
         model.bind(random_getter(model.tensors(), seed, spec.init_std, device=rt.device), rt)
         ps = page_size or getattr(cfg, "kv_page_size", None) or 16
         return cls(model, rt, ps, num_pages, max_requests, cuda_graphs)
@@ -148,6 +161,51 @@ class ModelRunner:
         Benchmarks use it to stand at a given context length without a prefill."""
         self.manager.reserve(rid, n_tokens)
         self.manager.commit(rid)
+
+    def reorder(self, groups: Sequence[Sequence[Hashable]], parents: Sequence[Sequence[int]], first: Sequence[Sequence[int]]) -> None:
+        """Requests of a group that go on from one another, all at once: request groups[g][b] takes over what request
+        groups[g][parents[g][b]] holds, cached keys and values from position first[g][b] on (below it the two are the same)
+        and per-request states.  Groups of equal size; the requests of a group have the same length."""
+        width = len(groups[0]) if groups else 0
+        if any(len(x) != width for part in (groups, parents, first) for x in part) or not len(groups) == len(parents) == len(first):
+            raise ValueError("reorder: groups, parents and first positions of different sizes")
+        rids = [rid for g in groups for rid in g]
+        if len(set(rids)) != len(rids):
+            raise ValueError("reorder: a request appears twice")
+        lengths = [self.manager.length(rid) for rid in rids]
+        if any(lengths[i] != lengths[i - i % width] for i in range(len(rids))):
+            raise ValueError("reorder: the requests of a group have different lengths")
+        if not rids or all(p == b for g in parents for b, p in enumerate(g)):
+            return
+        if any(not 0 <= p < width for g in parents for p in g):
+            raise ValueError(f"reorder: a parent outside 0..{width - 1}")
+        if self._page_sets is None:
+            tensors = [[] for _ in self.group_specs]
+            for c, r in zip(self.caches, self.model.cache_requests()):
+                if c is not None and c.write:
+                    tensors[c.group] += [c.k] if r.values_in_keys else [c.k, c.v]
+            self._page_sets = [ops.PageSet(t) for t in tensors]
+            states = [t for s in self.states for t in (s.values() if isinstance(s, dict) else () if s is None else (s,)) if t.numel()]
+            self._slot_set = ops.SlotSet(states) if states else None
+        # everything that the kernels read in one upload: parents | first | lengths | slots | a block table for each cache group
+        R, widths = len(rids), [max(1, max(self.manager.table_len(rid, g) for rid in rids)) for g in range(len(self.group_specs))]
+        host = np.full(4 * R + R * sum(widths), -1, dtype=np.int32)
+        host[:R], host[R:2 * R], host[2 * R:3 * R] = np.ravel(parents), np.ravel(first), lengths
+        host[3 * R:4 * R] = [self.manager.slot(rid) for rid in rids]
+        at, tables = 4 * R, []
+        for g, w in enumerate(widths):
+            block = host[at:at + R * w].reshape(R, w)
+            for i, rid in enumerate(rids):
+                row = self.manager.table_array(rid, g)
+                block[i, :len(row)] = row
+            tables.append(at)
+            at += R * w
+        dev = torch.from_numpy(host).to(self.rt.device)
+        d_parents = dev[:R].view(len(groups), width)
+        for pages, t, w in zip(self._page_sets, tables, widths):
+            ops.reorder_pages(pages, dev[t:t + R * w].view(R, w), d_parents, dev[R:2 * R], dev[2 * R:3 * R])
+        if self._slot_set is not None:
+            ops.reorder_slots(self._slot_set, dev[3 * R:4 * R], d_parents)
 
     def has_request(self, rid: Hashable) -> bool:
         return rid in self.manager.requests

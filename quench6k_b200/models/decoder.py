@@ -120,7 +120,7 @@ class DecoderModel:
                 part.bind(lambda n, pre=pre: get(pre + n), rt)
         self.final_norm.bind(lambda n: get(s.final_norm_prefix + n), rt)
         self.stream_sum = torch.ones(s.streams, dtype=torch.float32, device=rt.device) if s.streams else None
-        self.head = self.embed if s.head_name is None else to_operand(get(s.head_name), rt)
+        self.head = self.embed if s.head_name is None else linear.to_weight(get(s.head_name), rt)
 
     # ------------------------------------------------------------------ one step
     def forward(self, ctx, caches: List[Optional[LayerCache]], states: List[Optional[torch.Tensor]]) -> Optional[torch.Tensor]:

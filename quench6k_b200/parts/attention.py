@@ -33,7 +33,7 @@ import torch
 from .. import ops
 from ..spec import PartSpec, TensorSpec
 from . import linear
-from .base import (POSITION_ENCODINGS, CacheRequest, Mixer, make_part, register_mixer, to_f32, to_operand)
+from .base import (POSITION_ENCODINGS, CacheRequest, Mixer, make_part, register_mixer, to_f32)
 
 
 @register_mixer("attention")
@@ -142,8 +142,9 @@ class Attention(Mixer):
             self.w_qkv[self.g_col:self.g_col + self.Hq].copy_(get(n["gate"]))
         for name, lo, hi in ((n["q"], 0, nq), (n["k"], nq, nq + nk), (n["v"], nq + nk, nq + nk + nv))[:len(pieces)]:
             self.w_qkv[lo:hi].copy_(get(name))
+        self.w_qkv = linear.to_weight(self.w_qkv, rt)
         self.w_q = self.w_qkv if self.head_gate else self.w_qkv[:nq]      # what a layer that reads another's pages multiplies with
-        self.w_o = to_operand(get(n["o"]), rt)
+        self.w_o = linear.to_weight(get(n["o"]), rt)
         if self.qk_norm and self.qk_norm_weight:
             self.q_norm, self.k_norm = to_f32(get(n["q_norm"]), rt), to_f32(get(n["k_norm"]), rt)
         elif self.qk_norm:

@@ -40,6 +40,8 @@ class Runtime:
     device: torch.device
     dtype: torch.dtype                  # operand, activation and cache dtype: bfloat16, or float32 for the true 32-bit path
     tensor_cores: bool = True           # bfloat16 only: use the tcgen05 kernels where a shape allows
+    int8_weights: bool = False          # bfloat16 only: the matrices that parts bind through linear.to_weight are kept in 8 bits,
+                                        # and their products take the activations to 8 bits row by row
 
     @property
     def is_fp32(self) -> bool:

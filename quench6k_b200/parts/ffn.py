@@ -48,8 +48,8 @@ class DenseSwiGLU(FeedForward):
 
     def bind(self, get, rt):
         self.rt = rt
-        self.w_gate, self.w_up = to_operand(get(self.names["gate"]), rt), to_operand(get(self.names["up"]), rt)
-        self.w_down = to_operand(get(self.names["down"]), rt)
+        self.w_gate, self.w_up = linear.to_weight(get(self.names["gate"]), rt), linear.to_weight(get(self.names["up"]), rt)
+        self.w_down = linear.to_weight(get(self.names["down"]), rt)
 
     def _gated(self, xn):
         ops.current_tag = "dense.gate_up"
@@ -149,9 +149,12 @@ class RoutedExperts(FeedForward):
             self.w_router[self.total:self.total + 1].copy_(get(n["shared_gate"]))
         else:
             self.w_router = to_operand(get(n["router"]), rt)
-        self.w_up = to_operand(get(n["up"]), rt)
-        self.w_gate = to_operand(get(n["gate"]), rt) if self.gated else self.w_up      # ungated: the first (only) product's weights
-        self.w_down = to_operand(get(n["down"]), rt)
+        # in 8 bits all three, or none (both widths are rows of one of them)
+        self.int8 = rt.int8_weights and linear.int8_rows_allowed(self.D) and linear.int8_rows_allowed(self.I)
+        weight = linear.to_weight if self.int8 else to_operand
+        self.w_up = weight(get(n["up"]), rt)
+        self.w_gate = weight(get(n["gate"]), rt) if self.gated else self.w_up      # ungated: the first (only) product's weights
+        self.w_down = weight(get(n["down"]), rt)
         self.correction = to_f32(get(n["correction"]), rt) if self.has_correction else None
         if self.shared is not None:
             self.shared.bind(lambda n: get(self.shared_prefix + n), rt)
@@ -199,7 +202,7 @@ class RoutedExperts(FeedForward):
             return None
         pairs = T * self.k
         defer = defer and (self.shared is None or routed_only)
-        if (self.gated and self.act == "silu" and not self.own_router and rt.tensor_cores and not rt.is_fp32 and ops.router_small_supported(T, self.E, self.D, self.k)
+        if (not self.int8 and self.gated and self.act == "silu" and not self.own_router and rt.tensor_cores and not rt.is_fp32 and ops.router_small_supported(T, self.E, self.D, self.k)
                 and ops.tc_supported(xn, self.w_gate) and self.I % 8 == 0):
             # a decode step: router and top-k in one launch, then one weight tile stream per
             # (token, slot) pair straight from the selection, no permutation and no gather
@@ -234,7 +237,13 @@ class RoutedExperts(FeedForward):
             more = ()
         if self.routing_tap is not None:
             self._tap(ctx, sel_e, logits)
-        if (T <= self.pair_tokens and defer and rt.tensor_cores and not rt.is_fp32 and ops.tc_supported(xn, self.w_up) and self.I % 8 == 0):
+        if self.int8 and T <= self.pair_tokens and defer:
+            ops.current_tag = "experts.gate_up"
+            act = self.act if not self.gated or self.act != "silu" else None
+            first = linear.pair_products(xn, sel_e, self.k, self.w_gate, self.w_up if self.gated else None, act)     # [pairs, I]
+            ops.current_tag = "experts.down"
+            return self._rows(linear.pair_products(first, sel_e, 1, self.w_down), sel_w, None, xn, more)
+        if (not self.int8 and T <= self.pair_tokens and defer and rt.tensor_cores and not rt.is_fp32 and ops.tc_supported(xn, self.w_up) and self.I % 8 == 0):
             # a step of a few tokens whose router is not the one-launch kernel's: still one weight tile stream per
             # (token, slot) pair straight from the selection, no permutation and no gather
             ops.current_tag = "experts.gate_up"

@@ -1,2 +1,2 @@
-from .params import SamplingParams
+from .params import BeamParams, SamplingParams
 from .sampler import Sampler, SplitMix64, pick_from_pool, pool_size

@@ -43,3 +43,25 @@ class SamplingParams:
     @classmethod
     def greedy_params(cls, max_tokens: int = 64, stop_tokens=()) -> "SamplingParams":
         return cls(max_tokens=max_tokens, temperature=0.0, stop_tokens=list(stop_tokens))
+
+
+@dataclass
+class BeamParams:
+    """Options of a beam search.  A continuation's worth is the sum of its tokens' log-probabilities over its length (stop token
+    included) to the power length_penalty."""
+    width: int = 4                       # beams of a prompt
+    max_tokens: int = 64
+    length_penalty: float = 1.0          # 0: sums as they are; larger values favour long continuations
+    num_return: Optional[int] = None     # continuations that are returned; None: all of them (at most `width`)
+    early_stopping: bool = False         # end as soon as `width` continuations have ended, though a live beam might still become worth more
+    stop_tokens: List[int] = field(default_factory=list)   # a continuation ends with any of these (which belongs to it)
+
+    def validate(self) -> None:
+        if not 1 <= self.width <= 32:
+            raise ValueError("width must be in 1..32")
+        if self.max_tokens < 1:
+            raise ValueError("max_tokens must be at least 1")
+        if self.num_return is not None and not 1 <= self.num_return <= self.width:
+            raise ValueError("num_return must be in 1..width")
+        if self.width * (1 + len(set(self.stop_tokens))) > 128:
+            raise ValueError("width times one more than the number of stop tokens must be at most 128")
