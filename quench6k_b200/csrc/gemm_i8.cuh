@@ -2,8 +2,6 @@
 #pragma once
 #include "common.cuh"
 
-namespace {
-
 enum { I8_STORE = 0, I8_ADD = 1, I8_GATED = 2, I8_ACT = 4 };     // FP32 stored or added; bfloat16 act(v) * u, bfloat16 act(v)
 
 struct I8Args {
@@ -18,7 +16,11 @@ struct I8Args {
     int early;                     // the kernel before this one on the stream made a and a_scale and nothing else that is read here
     int epilogue, act;
     float act_param;
+    const __nv_bfloat16* x;        // not null: the rows of a and their scales are still to be made from these, row pitch ldx (few rows only)
+    long long ldx;
 };
+
+namespace {
 
 #define I8_OPERANDS                                                                                                                   \
     const void *a, long long lda, const float *a_scale, int rows, const void *w, const float *w_scale, const void *w2, const float *w2_scale, int N, int K, \
@@ -33,7 +35,7 @@ inline int i8_args(I8Args* p, const char* who, I8_OPERANDS) {
     Q6K_REQUIRE(act >= 0 && act <= (epi == I8_GATED ? Q6K_ACT_CLAMPED : 2), "%s: unknown activation %d", who, act);
     Q6K_REQUIRE(!(offsets && pair_expert) && groups >= 1 && pair_div >= 1, "%s: groups %d, pair_div %d", who, groups, pair_div);
     *p = I8Args{(const int8_t*)a, (const int8_t*)w, (const int8_t*)w2, a_scale, w_scale, w2_scale, a_rows, offsets, pair_expert, out, lda, ldo,
-                rows, N, K, groups, pair_div, early, epi, act, act_param};
+                rows, N, K, groups, pair_div, early, epi, act, act_param, nullptr, 0};
     return 0;
 }
 

@@ -8,12 +8,18 @@
 // activation row and hands them to two instructions as if they were the layout's pieces; the four lanes that share a row cover
 // 64 contiguous bytes.  A block's eight warps split K in turns, a warp has all its loads of a turn in flight at once, and the
 // warps' sums meet in shared memory.
+// Rows that come in bfloat16 and hold few values in all are taken to 8 bits by every block for itself (by the rule of quantize.cuh),
+// while its first weights are on their way: one launch instead of two.
 #include "common.cuh"
 #include "gemm_i8.cuh"
+#include "quantize.cuh"
 
 namespace {
 
 constexpr int R8_WARPS = 8, R8_ROWS = 16;
+#ifndef I8_HERE
+#define I8_HERE 16384
+#endif
 
 __device__ __forceinline__ void r8_mma(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -22,12 +28,19 @@ __device__ __forceinline__ void r8_mma(int* c, uint32_t a0, uint32_t a1, uint32_
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// grid: (blocks of 16 RB columns, 1 or pairs).  NB: blocks of 8 rows; RB: blocks of 16 columns; LOADS: 16-byte loads per lane and weight row in flight at once.
-template <bool DUAL, int NB, int RB, int LOADS>
+// Bytes between rows in shared memory: the eight lanes of two rows that are served at once read different banks.
+__host__ __device__ inline int r8_pitch(int K) { return (K + 127) / 128 * 128 + 64; }
+
+// grid: (blocks of 16 RB columns, 1 or pairs).  NB: blocks of 8 rows; RB: blocks of 16 columns; LOADS: 16-byte loads per lane and weight row in flight at once;
+// HERE: the rows are x in bfloat16, taken to 8 bits here.
+template <bool DUAL, int NB, int RB, int LOADS, bool HERE>
 __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Args p) {
     pdl_launch();
     constexpr int MATS = DUAL ? 2 : 1, TURN = 64 * LOADS;
     __shared__ int meet[R8_WARPS][MATS * RB * NB * 4 * 32];
+    __shared__ unsigned most[HERE ? R8_ROWS : 1][R8_WARPS];
+    __shared__ float scale[HERE ? R8_ROWS : 1];
+    extern __shared__ __align__(16) int8_t rows8[];       // HERE: [rows, pitch]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, pair = lane & 3;
     const int n0 = blockIdx.x * RB * 16, row0 = blockIdx.y, rows = p.pair_expert ? 1 : p.rows;
     if (!p.early) pdl_wait();
@@ -48,10 +61,42 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
             if (DUAL) wrow[1][rb][h] = p.w2 + r * p.K + pair * 16;
         }
     auto source = [&](int r) -> long long { return p.pair_expert ? r / p.pair_div : p.a_rows ? p.a_rows[r] : r; };
+    // every thread of the block once: the rows in 8 bits to shared memory
+    auto take_rows = [&] {
+        if constexpr (HERE) {
+            for (int r = 0; r < rows; ++r) {
+                const __nv_bfloat16* from = p.x + source(row0 + r) * p.ldx;
+                unsigned m = 0;
+                for (int k = threadIdx.x * 8; k < p.K; k += R8_WARPS * 256) {
+                    Piece<__nv_bfloat16, 8> v;
+                    v.take(ld_after_wait(from + k));
+                    m = max(m, v.most());
+                }
+                m = __reduce_max_sync(0xffffffffu, m);
+                if (lane == 0) most[r][warp] = m;
+            }
+            __syncthreads();
+            for (int r = 0; r < rows; ++r) {
+                unsigned m = 0;
+#pragma unroll
+                for (int q = 0; q < R8_WARPS; ++q) m = max(m, most[r][q]);
+                const RowScale s = row_scale(m);
+                if (threadIdx.x == 0) scale[r] = s.scale;
+                const __nv_bfloat16* from = p.x + source(row0 + r) * p.ldx;
+                for (int k = threadIdx.x * 8; k < p.K; k += R8_WARPS * 256) {
+                    Piece<__nv_bfloat16, 8> v;
+                    v.take(ld_after_wait(from + k));
+                    v.store(rows8 + r * r8_pitch(p.K) + k, s.up);
+                }
+            }
+            __syncthreads();
+        }
+    };
     const int8_t* xrow[NB];
-    bool live[NB], waited = false;
+    bool live[NB], first_turn = true;
     int acc[MATS][RB][NB][4] = {};
-    for (int k0 = warp * TURN; k0 < p.K; k0 += R8_WARPS * TURN) {
+    int k0 = warp * TURN;
+    do {                                                  // (a warp without a turn of its own loads nothing in its first one)
         uint4 w[MATS][RB][2][LOADS], x[NB][LOADS];
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
@@ -64,20 +109,22 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
 #pragma unroll
                     for (int h = 0; h < 2; ++h) w[m][rb][h][j] = in ? ld_once(wrow[m][rb][h] + k, once) : make_uint4(0, 0, 0, 0);
         }
-        if (!waited) {
+        if (first_turn) {
+            first_turn = false;
             if (p.early) pdl_wait();
-            waited = true;
+            if constexpr (HERE) take_rows();
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 live[nb] = nb * 8 + quad < rows;
-                xrow[nb] = p.a + source(live[nb] ? row0 + nb * 8 + quad : row0) * p.lda + pair * 16;
+                if (HERE) xrow[nb] = rows8 + (live[nb] ? nb * 8 + quad : 0) * r8_pitch(p.K) + pair * 16;
+                else xrow[nb] = p.a + source(live[nb] ? row0 + nb * 8 + quad : row0) * p.lda + pair * 16;
             }
         }
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int k = k0 + j * 64;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) x[nb][j] = k + pair * 16 < p.K && live[nb] ? ld_after_wait(xrow[nb] + k) : make_uint4(0, 0, 0, 0);
+            for (int nb = 0; nb < NB; ++nb) x[nb][j] = k + pair * 16 >= p.K || !live[nb] ? make_uint4(0, 0, 0, 0) : HERE ? *(const uint4*)(xrow[nb] + k) : ld_after_wait(xrow[nb] + k);
         }
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
@@ -91,8 +138,8 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
                         r8_mma(acc[m][rb][nb], lo.x, hi.x, lo.y, hi.y, t.x, t.y);
                         r8_mma(acc[m][rb][nb], lo.z, hi.z, lo.w, hi.w, t.z, t.w);
                     }
-    }
-    if (!waited && p.early) pdl_wait();                   // a warp without a turn of its own
+        k0 += R8_WARPS * TURN;
+    } while (k0 < p.K);
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
 #pragma unroll
@@ -112,7 +159,7 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
             s += meet[q][idx];
             if (DUAL) s2 += meet[q][RB * NB * 4 * 32 + idx];
         }
-        const float xs = p.a_scale[source(row0 + r)];
+        const float xs = HERE ? scale[r] : p.a_scale[source(row0 + r)];
         const float v = (float)s * (xs * p.w_scale[first + n]);
         const float u = DUAL ? (float)s2 * (xs * p.w2_scale[first + n]) : 0.0f;
         i8_store<DUAL>(p, (long long)(row0 + r) * p.ldo + n, v, u);
@@ -121,21 +168,18 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
 
 template <bool DUAL, int NB, int RB, int LOADS>
 void launch(const I8Args& p, int pairs, cudaStream_t st) {
-    q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS>, dim3((p.N + RB * 16 - 1) / (RB * 16), pairs), R8_WARPS * 32, 0, st, p);
+    const dim3 grid((p.N + RB * 16 - 1) / (RB * 16), pairs);
+    if (p.x) q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS, true>, grid, R8_WARPS * 32, (p.pair_expert ? 1 : p.rows) * r8_pitch(p.K), st, p);
+    else q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS, false>, grid, R8_WARPS * 32, 0, st, p);
 }
 
-}  // namespace
-
-// See ops.gemm_i8 and ops.linear_i8 for the operands: up to 16 rows, or any number of pairs.
-Q6K_API int q6k_gemm_i8_rows(I8_OPERANDS, cudaStream_t st) {
-    I8Args p;
-    if (int rc = i8_args(&p, "gemm_i8_rows", I8_NAMES)) return rc;
+int launch_rows(const I8Args& p, cudaStream_t st) {
     if (p.rows == 0) return 0;
-    Q6K_REQUIRE(!offsets && rows <= (pair_expert ? 65535 : R8_ROWS), "gemm_i8_rows: %d rows", rows);
-    const int pairs = pair_expert ? rows : 1, row_blocks = pair_expert || rows <= 8 ? 1 : 2;
+    Q6K_REQUIRE(!p.offsets && p.rows <= (p.pair_expert ? 65535 : R8_ROWS), "gemm_i8_rows: %d rows", p.rows);
+    const int pairs = p.pair_expert ? p.rows : 1, row_blocks = p.pair_expert || p.rows <= 8 ? 1 : 2;
     // 32 columns a block where that leaves every SM two of them; long rows of few blocks: eight loads a row at once
-    const bool wide = (long long)N * pairs >= 148 * 2 * 32, deep = K >= 8192 && !wide;
-    if (w2) {
+    const bool wide = (long long)p.N * pairs >= 148 * 2 * 32, deep = p.K >= 8192 && !wide;
+    if (p.w2) {
         if (row_blocks == 1) launch<true, 1, 1, 4>(p, pairs, st);
         else launch<true, 2, 1, 4>(p, pairs, st);
     } else if (row_blocks == 1) {
@@ -147,4 +191,43 @@ Q6K_API int q6k_gemm_i8_rows(I8_OPERANDS, cudaStream_t st) {
         else launch<false, 2, 1, 4>(p, pairs, st);
     }
     return q6k_check_launch("gemm_i8_rows");
+}
+
+}  // namespace
+
+int q6k_quantize_rows_launch(const void* x, long long ldx, int R, int K, int dtype, void* q, float* scale, cudaStream_t st);
+int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st);
+
+// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered, gathered_scale: int8 [rows, K] and FP32 [rows] of scratch, where a_rows comes with
+// more than 16 rows or with groups.  tile: see q6k_gemm_i8_tc_launch (0 but for measurements).
+Q6K_API int q6k_gemm_i8(I8_OPERANDS, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st) {
+    I8Args p;
+    if (int rc = i8_args(&p, "gemm_i8", I8_NAMES)) return rc;
+    Q6K_REQUIRE(!pair_expert, "gemm_i8: pairs come with rows that are not in 8 bits");
+    if (rows <= R8_ROWS && !offsets && tile == 0) return launch_rows(p, st);
+    return q6k_gemm_i8_tc_launch(p, a_total, gathered, gathered_scale, tile, st);
+}
+
+// Values of bfloat16 rows up to which every block takes them to 8 bits itself.
+static bool taken_here(int T, int K, bool pairs) { return pairs ? K <= 8192 : (long long)T * K <= I8_HERE; }
+
+// Bytes of scratch that q6k_linear_i8 takes.
+Q6K_API long long q6k_linear_i8_scratch(int T, int K) { return (long long)T * K + 4LL * T; }
+
+// See ops.linear_i8: x of dtype code, T rows of pitch ldx; a, lda and a_scale of the operands are not looked at, and `early` says that the weights and
+// the pair list are older than the kernel before this call.  scratch: 16-byte aligned.
+Q6K_API int q6k_linear_i8(const void* x, long long ldx, int T, int dtype, void* scratch, I8_OPERANDS, cudaStream_t st) {
+    I8Args p;
+    if (int rc = i8_args(&p, "linear_i8", scratch, K, (const float*)((char*)scratch + (long long)T * K), rows, w, w_scale, w2, w2_scale, N, K, a_rows, offsets, groups, pair_expert,
+                         pair_div, out, ldo, epilogue, act_param, 1))
+        return rc;
+    Q6K_REQUIRE(!offsets && !a_rows && (pair_expert ? (rows + pair_div - 1) / pair_div <= T : rows == T), "linear_i8: %d rows of %d", rows, T);
+    if (rows == 0) return 0;
+    const bool few = pair_expert || rows <= R8_ROWS;
+    if (few && dtype == Q6K_BF16 && ldx % 8 == 0 && ((uintptr_t)x & 15) == 0 && taken_here(T, K, pair_expert != nullptr)) {
+        p.x = (const __nv_bfloat16*)x, p.ldx = ldx, p.early = early;
+        return launch_rows(p, st);
+    }
+    if (int rc = q6k_quantize_rows_launch(x, ldx, T, K, dtype, scratch, (float*)p.a_scale, st)) return rc;
+    return few ? launch_rows(p, st) : q6k_gemm_i8_tc_launch(p, T, nullptr, nullptr, 0, st);
 }

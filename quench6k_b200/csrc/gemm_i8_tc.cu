@@ -515,22 +515,21 @@ Q6K_API int q6k_gemm_i8_status() {
     return v;
 }
 
-// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered, gathered_scale (with a_rows): int8 [rows, K] and FP32 [rows] of scratch.
-// tile: rows of a tile, negative for pairs of CTAs (0: chosen here).
-Q6K_API int q6k_gemm_i8_tc(I8_OPERANDS, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st) {
-    TcArgs t;
-    if (int rc = i8_args(&t.p, "gemm_i8", I8_NAMES)) return rc;
-    if (rows == 0) return 0;
-    Q6K_REQUIRE(!pair_expert && groups <= MAX_GROUPS && (long long)groups * N < (1LL << 31) - 256, "gemm_i8: %d groups (at most %d) of %d columns", groups, MAX_GROUPS, N);
-    if (a_rows) {
+// More than a few rows, or groups.  gathered, gathered_scale (with a_rows): int8 [rows, K] and FP32 [rows] of scratch.  tile: rows of a tile, negative for
+// pairs of CTAs (0: chosen here).
+int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st) {
+    TcArgs t{p};
+    if (p.rows == 0) return 0;
+    Q6K_REQUIRE(p.groups <= MAX_GROUPS && (long long)p.groups * p.N < (1LL << 31) - 256, "gemm_i8: %d groups (at most %d) of %d columns", p.groups, MAX_GROUPS, p.N);
+    if (p.a_rows) {
         Q6K_REQUIRE(gathered && gathered_scale && ((uintptr_t)gathered & 15) == 0, "gemm_i8: no scratch for the rows that are picked");
-        q6k_launch(gather_i8_kernel, (rows + 7) / 8, 256, 0, st, t.p.a, lda, a_scale, a_rows, rows, K, (int8_t*)gathered, gathered_scale);
+        q6k_launch(gather_i8_kernel, (p.rows + 7) / 8, 256, 0, st, p.a, p.lda, p.a_scale, p.a_rows, p.rows, p.K, (int8_t*)gathered, gathered_scale);
         if (int rc = q6k_check_launch("gemm_i8: gather")) return rc;
-        t.p.a = (const int8_t*)gathered, t.p.a_scale = gathered_scale, t.p.a_rows = nullptr, t.p.lda = K, t.p.early = 1;
-        a_total = rows;
+        t.p.a = (const int8_t*)gathered, t.p.a_scale = gathered_scale, t.p.a_rows = nullptr, t.p.lda = p.K, t.p.early = 1;
+        a_total = p.rows;
     }
-    Q6K_REQUIRE(a_total >= rows, "gemm_i8: %d rows of %d", rows, a_total);
-    const bool dual = w2 != nullptr;
+    Q6K_REQUIRE(a_total >= p.rows, "gemm_i8: %d rows of %d", p.rows, a_total);
+    const bool dual = p.w2 != nullptr;
     if (tile == 0) tile = choose_tile(t.p, dual);
 #define GO(T_, BT_, CTAS_) \
     case T_: return dual ? launch<BT_, CTAS_, true>(t, a_total, st) : launch<BT_, CTAS_, false>(t, a_total, st)

@@ -62,6 +62,7 @@ launch_count = 0
 
 
 _functions = {}
+_ARGTYPES = {}                              # launchers that are called with plain numbers instead of ctypes objects
 
 # Where a step's time goes, without a profiler (the reference times its forward pass op by op the same way and can
 # synchronise after every op: crates/engine/src/profile.rs:1-55, crates/engine/src/flint.rs:685-697).
@@ -98,6 +99,8 @@ def _call(fn_name: str, *args, launches: Optional[int] = None):
     if fn is None:
         fn = _functions[fn_name] = getattr(library(), fn_name)
         fn.restype = ctypes.c_int
+        if fn_name in _ARGTYPES:
+            fn.argtypes = _ARGTYPES[fn_name]
     if _profile is not None:
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
@@ -2037,19 +2040,53 @@ def hyper_step(x: torch.Tensor, S: int, add=None, read=None, rows: Optional[torc
 
 
 # --------------------------------------------------------------------------- products in 8-bit integers
-def _need_here(t: torch.Tensor, name: str):
-    """The kernels run on the current device's stream: an operand on another device would be read there."""
-    if not t.is_cuda:
-        raise KernelError(f"{name} is on {t.device}; the kernels run on a CUDA device only")
-    if t.device.index != torch.cuda.current_device():
-        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+# The launchers below are called with plain numbers (a ctypes object for each argument is what takes most of a short call's host time).
+_p, _t = ctypes.c_void_p, ctypes.c_int
+_I8_OPERANDS = [_p, _ll, _p, _t, _p, _p, _p, _p, _t, _t, _p, _p, _t, _p, _t, _p, _ll, _t, _f, _t]
+_ARGTYPES.update({
+    "q6k_quantize_rows": [_p, _ll, _t, _t, _t, _p, _p, _p],
+    "q6k_gemm_i8": _I8_OPERANDS + [_t, _p, _p, _t, _p],
+    "q6k_linear_i8": [_p, _ll, _t, _t, _p] + _I8_OPERANDS + [_p],
+    "q6k_beam_select": [_p, _p, _t, _t, _t, _t, _p, _ll, _p, _p, _p, _p],
+    "q6k_reorder_pages": [_t, _p, _p, _p, _p, _p, _t, _t, _t, _t, _p, _p, _p, _p],
+    "q6k_reorder_slots": [_t, _p, _p, _p, _p, _t, _t, _p, _p],
+})
 
 
-def _need_rows(t: torch.Tensor, name: str):
-    """A matrix whose rows may lie apart."""
-    _need_here(t, name)
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _here(*operands) -> int:
+    """The current device, on which every operand has to be: the kernels run on its current stream."""
+    for name, t in operands:
+        if not t.is_cuda:
+            raise KernelError(f"{name} is on {t.device}; the kernels run on a CUDA device only")
+    device = _current_device()
+    for name, t in operands:
+        if t.get_device() != device:
+            raise KernelError(f"{name} is on {t.device}, the current device is cuda:{device}")
+    return device
+
+
+def _is(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
+    """Type, shape and contiguity (what _need says, for operands that _here has seen)."""
+    if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise KernelError(f"{name} is {t.dtype} {tuple(t.shape)}{'' if t.is_contiguous() else ', not contiguous'}, expected {dtype} {tuple(shape)}")
+
+
+def _row_pitch(t: torch.Tensor, name: str) -> int:
+    """The pitch of a matrix whose rows may lie apart."""
+    if t.dim() != 2:
+        raise KernelError(f"{name} has shape {tuple(t.shape)}, expected rows")
+    (rows, cols), (pitch, step) = t.shape, t.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and pitch < cols):
         raise KernelError(f"{name} has shape {tuple(t.shape)} and strides {tuple(t.stride())}, expected rows of neighbouring values")
+    return pitch if rows > 1 else cols
 
 
 def quantize_rows(x: torch.Tensor):
@@ -2058,48 +2095,53 @@ def quantize_rows(x: torch.Tensor):
     for q * scale.  A row of zeros (or of values below 3.8e-37, where u is infinite) has the scale 0; a row with a value that is
     not finite has zeros and the scale NaN."""
     code = dtype_code(x.dtype)
-    _need_rows(x, "x")
+    device = _here(("x", x))
+    pitch = _row_pitch(x, "x")
     R, K = x.shape
-    if K < 1:
-        raise KernelError("quantize_rows: rows without values")
+    if K < 1 or R > 2 ** 31 - 1 or K > 2 ** 31 - 1:
+        raise KernelError(f"quantize_rows: {R} rows of {K} values")
     q = torch.empty((R, K), dtype=torch.int8, device=x.device)
-    scale = torch.empty(R, dtype=torch.float32, device=x.device)
-    _call("q6k_quantize_rows", _ptr(x), _ll(x.stride(0) if R > 1 else K), _i(R), _i(K), _i(code), _ptr(q), _ptr(scale), _stream())
+    scale = torch.empty((R,), dtype=torch.float32, device=x.device)
+    _call("q6k_quantize_rows", x.data_ptr(), pitch, R, K, code, q.data_ptr(), scale.data_ptr(), _stream_of(device), launches=1 if R else 0)
     return q, scale
 
 
-def _i8_weights(w, w_scale, w2, w2_scale, K: int, grouped: bool, who: str):
-    """The checks that gemm_i8 and linear_i8 share; (matrices, N)."""
-    _need_here(w, "w")
-    _need(w, "w", torch.int8)
-    if w.dim() != (3 if grouped else 2) or w.shape[-1] != K:
-        raise KernelError(f"{who}: rows of {K} against w of shape {tuple(w.shape)} (three dimensions go with offsets or pair_expert)")
+def _i8_product(w, w_scale, w2, w2_scale, K: int, grouped: bool, accumulate: bool, act, out, rows: int, who: str):
+    """The checks that gemm_i8 and linear_i8 share: (matrices, columns, epilogue, output)."""
+    shape = w.shape
+    if w.dtype is not torch.int8 or len(shape) != (3 if grouped else 2) or shape[-1] != K or not w.is_contiguous():
+        raise KernelError(f"{who}: rows of {K} against w, {w.dtype} {tuple(shape)} (contiguous int8; three dimensions go with offsets or pair_expert)")
     if K % 16 or not 0 < K < 131072 or w.data_ptr() % 16:
         raise KernelError(f"{who}: K={K} must be a multiple of 16 below 131072 and w start on 16 bytes")
-    _need(w_scale, "w_scale", torch.float32, w.shape[:-1])
+    _is(w_scale, "w_scale", torch.float32, shape[:-1])
     if (w2 is None) != (w2_scale is None):
         raise KernelError(f"{who}: the second matrix and its scales go together")
     if w2 is not None:
-        _need(w2, "w2", torch.int8, w.shape)
-        _need(w2_scale, "w2_scale", torch.float32, w.shape[:-1])
+        _is(w2, "w2", torch.int8, shape)
+        _is(w2_scale, "w2_scale", torch.float32, shape[:-1])
         if w2.data_ptr() % 16:
             raise KernelError(f"{who}: w2 must start on 16 bytes")
-    return (w.shape[0] if grouped else 1), w.shape[-2]
-
-
-def _i8_out(out, rows: int, N: int, epi: int, device, who: str):
-    dtype = torch.float32 if (epi & 255) in (EPI_STORE, EPI_ADD) else torch.bfloat16
+        if accumulate:
+            raise KernelError(f"{who}: a gated product is stored, not added")
+    N, epi = shape[-2], _epilogue(w2, accumulate, act)
+    dtype = torch.float32 if epi in (EPI_STORE, EPI_ADD) else torch.bfloat16
+    if N < 1 or rows > 2 ** 31 - 1:
+        raise KernelError(f"{who}: {rows} rows, {N} columns")
     if out is None:
-        if (epi & 255) == EPI_ADD:
+        if accumulate:
             raise KernelError(f"{who}: accumulate needs an output")
-        return torch.empty((rows, N), dtype=dtype, device=device)
-    _need(out, "out", dtype)
-    if out.dim() != 2 or out.shape[0] < rows or out.shape[1] != N:
-        raise KernelError(f"{who}: out has shape {tuple(out.shape)}, needs [{rows}, {N}]")
-    return out
+        out = torch.empty((rows, N), dtype=dtype, device=w.device)
+    elif out.dtype is not dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != N or not out.is_contiguous():
+        raise KernelError(f"{who}: out is {out.dtype} {tuple(out.shape)}, needs contiguous {dtype} [{rows}, {N}]")
+    return (shape[0] if grouped else 1), N, epi, out
 
 
-_i8_tile = 0
+def _data(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+_I8_FEW_ROWS = 16                        # products of at most this many rows take the kernel that streams weights past mma.sync
+_i8_tile = 0                             # rows of a tile for measurements (0: the library's rule)
 
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -2107,70 +2149,76 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
             offsets: Optional[torch.Tensor] = None, a_rows: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
     """y[r, n] = a_scale[r] * w_scale[n] * sum_k a[r, k] w[n, k] of int8 operands, the sum exact in 32-bit integers.
 
-    a: int8 [*, K], a_scale: float32 [*]; w: int8 [N, K] with w_scale float32 [N].  Stored in float32, or added into `out`
-    (accumulate).  With w2 the gated epilogue act(y) * y2 (act None: silu), with act alone act(y); both leave in bfloat16.
+    a: int8 [*, K] (its rows may lie apart), a_scale: float32 [*]; w: int8 [N, K] with w_scale float32 [N]; K a multiple of 16 below
+    131,072.  Stored in float32, or added into `out` (accumulate).  With w2 the gated epilogue act(y) * y2 (act None: silu), with
+    act alone act(y); both leave in bfloat16.
     a_rows (int32 [rows]): row r of the product is row a_rows[r] of a.  offsets (int32 [G + 1], ascending from 0) with w [G, N, K]
     and w_scale [G, N]: rows offsets[g] .. offsets[g + 1] - 1 go against matrix g; rows behind the last offset are left as they were.
     early: the caller's word that the kernel before this call made a and a_scale and nothing else that is read here: the weights
     are then fetched while it ends."""
-    _need_rows(a, "a")
-    if a.dtype != torch.int8:
+    if a.dtype is not torch.int8:
         raise KernelError(f"a has dtype {a.dtype}, expected torch.int8")
-    total, K = a.shape
-    _need(a_scale, "a_scale", torch.float32, (total,))
-    if a.data_ptr() % 16 or (total > 1 and a.stride(0) % 16):
-        raise KernelError("gemm_i8: the rows of a must start on 16 bytes")
     grouped = offsets is not None
-    groups, N = _i8_weights(w, w_scale, w2, w2_scale, K, grouped, "gemm_i8")
-    epi = _epilogue(w2, accumulate, act)
-    if accumulate and w2 is not None:
-        raise KernelError("gemm_i8: a gated product is stored, not added")
+    operands = [("a", a), ("a_scale", a_scale), ("w", w), ("w_scale", w_scale)]
+    operands += [(n, t) for n, t in (("w2", w2), ("w2_scale", w2_scale), ("out", out), ("offsets", offsets), ("a_rows", a_rows)) if t is not None]
+    device = _here(*operands)
+    lda = _row_pitch(a, "a")
+    total, K = a.shape
+    _is(a_scale, "a_scale", torch.float32, (total,))
+    if a_rows is not None:
+        _is(a_rows, "a_rows", torch.int32, (a_rows.numel(),))
+    rows = total if a_rows is None else a_rows.numel()
+    groups, N, epi, out = _i8_product(w, w_scale, w2, w2_scale, K, grouped, accumulate, act, out, rows, "gemm_i8")
+    if a.data_ptr() % 16 or lda % 16:
+        raise KernelError("gemm_i8: the rows of a must start on 16 bytes")
     if grouped:
-        _need(offsets, "offsets", torch.int32, (groups + 1,))
-    if a_rows is not None:
-        _need(a_rows, "a_rows", torch.int32)
-    rows = a_rows.numel() if a_rows is not None else total
-    out = _i8_out(out, rows, N, epi, a.device, "gemm_i8")
-    lda = a.stride(0) if total > 1 else K
-    if rows <= 16 and not grouped:
-        _call("q6k_gemm_i8_rows", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-              _ptr(a_rows), _ptr(None), _i(1), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(early), _stream())
-        return out
+        _is(offsets, "offsets", torch.int32, (groups + 1,))
     gathered = gathered_scale = None
-    if a_rows is not None:
+    if a_rows is not None and (grouped or rows > _I8_FEW_ROWS or _i8_tile):
         gathered, gathered_scale = torch.empty((rows, K), dtype=torch.int8, device=a.device), torch.empty(rows, dtype=torch.float32, device=a.device)
-    _call("q6k_gemm_i8_tc", _ptr(a), _ll(lda), _ptr(a_scale), _i(rows), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-          _ptr(a_rows), _ptr(offsets), _i(groups), _ptr(None), _i(1), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(early), _i(total), _ptr(gathered),
-          _ptr(gathered_scale), _i(_i8_tile), _stream(), launches=(rows > 0) * (1 if a_rows is None else 2))
+    _call("q6k_gemm_i8", a.data_ptr(), lda, a_scale.data_ptr(), rows, w.data_ptr(), w_scale.data_ptr(), _data(w2), _data(w2_scale), N, K, _data(a_rows), _data(offsets),
+          groups, 0, 1, out.data_ptr(), N, epi, _act_param(act), early, total, _data(gathered), _data(gathered_scale), _i8_tile, _stream_of(device),
+          launches=0 if rows == 0 else 1 if gathered is None else 2)
     return out
 
 
 def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool = False,
               w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None, pair_expert: Optional[torch.Tensor] = None,
-              pair_div: int = 1) -> torch.Tensor:
-    """The product of quantize_rows(x) with weights in 8 bits: x float32 or bfloat16 [T, K], the rest as in gemm_i8.  With
-    pair_expert (int32 [pairs]) and w [experts, N, K]: row y of the result is row y // pair_div of x against the matrix of expert
-    pair_expert[y]; a pair that names no matrix is left as it was."""
-    q, scale = quantize_rows(x)
-    if pair_expert is None:
-        return gemm_i8(q, scale, w, w_scale, out=out, accumulate=accumulate, w2=w2, w2_scale=w2_scale, act=act, early=True)
+              pair_div: int = 1, weights_are_old: bool = False) -> torch.Tensor:
+    """The product of quantize_rows(x) with weights in 8 bits: x float32 or bfloat16 [T, K] (its rows may lie apart), the rest as in
+    gemm_i8.  With pair_expert (int32 [pairs], at most 65,535) and w [experts, N, K]: row y of the result is row y // pair_div of x
+    against the matrix of expert pair_expert[y]; a pair that names no matrix is left as it was.
+    weights_are_old: the caller's word that the weights and the pair list were written before the kernel that precedes this call
+    on the stream started: they may then be fetched while it ends (a model's weights; they are not, if the call follows the
+    kernel that made them)."""
+    code = dtype_code(x.dtype)
+    operands = [("x", x), ("w", w), ("w_scale", w_scale)]
+    operands += [(n, t) for n, t in (("w2", w2), ("w2_scale", w2_scale), ("out", out), ("pair_expert", pair_expert)) if t is not None]
+    device = _here(*operands)
+    pitch = _row_pitch(x, "x")
     T, K = x.shape
-    groups, N = _i8_weights(w, w_scale, w2, w2_scale, K, True, "linear_i8")
-    _need(pair_expert, "pair_expert", torch.int32)
-    pairs = pair_expert.numel()
-    if pair_div < 1 or -(-pairs // pair_div) > T or pairs > 65535:
-        raise KernelError(f"linear_i8: {pairs} pairs (at most 65535), {pair_div} for each of {T} rows")
-    epi = _epilogue(w2, accumulate, act)
-    if accumulate and w2 is not None:
-        raise KernelError("linear_i8: a gated product is stored, not added")
-    out = _i8_out(out, pairs, N, epi, x.device, "linear_i8")
-    _call("q6k_gemm_i8_rows", _ptr(q), _ll(K), _ptr(scale), _i(pairs), _ptr(w), _ptr(w_scale), _ptr(w2), _ptr(w2_scale), _i(N), _i(K),
-          _ptr(None), _ptr(None), _i(groups), _ptr(pair_expert), _i(pair_div), _ptr(out), _ll(N), _i(epi), _f(_act_param(act)), _i(1), _stream())
+    pairs = 0 if pair_expert is None else pair_expert.numel()
+    if pair_expert is not None:
+        _is(pair_expert, "pair_expert", torch.int32, (pairs,))
+        if pair_div < 1 or -(-pairs // pair_div) > T or pairs > 65535:
+            raise KernelError(f"linear_i8: {pairs} pairs (at most 65535), {pair_div} for each of {T} rows")
+    rows = T if pair_expert is None else pairs
+    groups, N, epi, out = _i8_product(w, w_scale, w2, w2_scale, K, pair_expert is not None, accumulate, act, out, rows, "linear_i8")
+    scratch = torch.empty(T * K + 4 * T, dtype=torch.uint8, device=x.device)
+    _call("q6k_linear_i8", x.data_ptr(), pitch, T, code, scratch.data_ptr(), 0, K, 0, rows, w.data_ptr(), w_scale.data_ptr(), _data(w2), _data(w2_scale), N, K, 0, 0,
+          groups, _data(pair_expert), pair_div, out.data_ptr(), N, epi, _act_param(act), weights_are_old, _stream_of(device), launches=2 if rows else 0)
     return out
 
 
 # --------------------------------------------------------------------------- beam search
 BEAM_MAX_WIDTH, BEAM_MAX_COUNT = 32, 128
+
+
+@functools.lru_cache(maxsize=None)          # a question about sizes: asked of the library once
+def _beam_scratch(rows: int, V: int, count: int) -> int:
+    lib = library()
+    lib.q6k_beam_scratch.restype = ctypes.c_longlong
+    return lib.q6k_beam_scratch(_i(rows), _i(V), _i(count))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int):
@@ -2179,25 +2227,20 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int):
     among equals.  logits: float32 [requests * width, V], a request's beams in neighbouring rows; scores: float32 [requests, width].
     A continuation whose beam's score, logit or row sum is not finite counts as -infinity and comes after all others (a beam
     of score -infinity takes no part while others have continuations left).  t is compared in 64 bits and rounded on the way out."""
-    _need_here(logits, "logits")
-    _need(logits, "logits", torch.float32)
-    _need(scores, "scores", torch.float32)
-    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
+    device = _here(("logits", logits), ("scores", scores))
+    if scores.dim() != 2 or logits.dim() != 2:
         raise KernelError(f"beam_select: logits {tuple(logits.shape)} for scores {tuple(scores.shape)}")
-    requests, width = scores.shape
-    V = logits.shape[1]
-    count = int(count)
-    if not 1 <= width <= BEAM_MAX_WIDTH or not 1 <= count <= min(BEAM_MAX_COUNT, width * V) or width * V >= 1 << 31 or requests * width > 65535:
+    (requests, width), (rows, V), count = scores.shape, logits.shape, int(count)
+    _is(logits, "logits", torch.float32, (requests * width, V))
+    _is(scores, "scores", torch.float32, (requests, width))
+    if not 1 <= width <= BEAM_MAX_WIDTH or not 1 <= count <= min(BEAM_MAX_COUNT, width * V) or width * V >= 1 << 31 or rows > 65535:
         raise KernelError(f"beam_select: {count} continuations (1 to {BEAM_MAX_COUNT}) of {requests} requests of {width} beams (1 to {BEAM_MAX_WIDTH}) over {V} tokens")
-    lib = library()
-    lib.q6k_beam_scratch.restype = ctypes.c_longlong
-    nbytes = lib.q6k_beam_scratch(_i(requests * width), _i(V), _i(count))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    nbytes = _beam_scratch(rows, V, count) if rows else 0
     out = torch.empty((requests, count), dtype=torch.float32, device=logits.device)
-    where = torch.empty((2, requests, count), dtype=torch.int32, device=logits.device)
-    beams, tokens = where.unbind(0)
-    _call("q6k_beam_select", _ptr(logits), _ptr(scores), _i(requests), _i(width), _i(V), _i(count), _ptr(scratch), _ll(nbytes), _ptr(out), _ptr(beams), _ptr(tokens),
-          _stream(), launches=2 if requests else 0)
+    beams, tokens = torch.empty((2, requests, count), dtype=torch.int32, device=logits.device).unbind(0)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    _call("q6k_beam_select", logits.data_ptr(), scores.data_ptr(), requests, width, V, count, scratch.data_ptr(), nbytes, out.data_ptr(), beams.data_ptr(), tokens.data_ptr(),
+          _stream_of(device), launches=2 if rows else 0)
     return out, beams, tokens
 
 
@@ -2237,12 +2280,12 @@ class SlotSet:
                      (ctypes.c_longlong * n)(*[t.numel() // t.shape[0] * t.element_size() for t in self.tensors]))
 
 
-def _parents(parents: torch.Tensor, who: str):
-    _need_here(parents, "parents")
-    _need(parents, "parents", torch.int32)
-    if parents.dim() != 2 or not 1 <= parents.shape[1] <= BEAM_MAX_WIDTH or parents.shape[0] > 65535:
-        raise KernelError(f"{who}: parents have shape {tuple(parents.shape)}, expected [groups, 1 to {BEAM_MAX_WIDTH}]")
-    return parents.shape
+def _groups_of(parents: torch.Tensor, who: str):
+    shape = parents.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= BEAM_MAX_WIDTH or shape[0] > 65535:
+        raise KernelError(f"{who}: parents have shape {tuple(shape)}, expected [groups, 1 to {BEAM_MAX_WIDTH}]")
+    _is(parents, "parents", torch.int32, shape)
+    return shape
 
 
 def _batches(args, most: int = 128):
@@ -2259,28 +2302,30 @@ def reorder_pages(pages, table: torch.Tensor, parents: torch.Tensor, first: torc
     logical block, -1 where none is held (what a row does not hold stays as it is); parents: int32 [groups, width], a number
     within the group for each of its neighbouring rows (its own, or one outside the group: the row stays); first, lengths: int32
     [rows].  Pages that are written belong to one row only."""
+    device = _here(("table", table), ("parents", parents), ("first", first), ("lengths", lengths))
     if not isinstance(pages, PageSet):
         pages = PageSet(pages)
-    groups, width = _parents(parents, "reorder_pages")
+    groups, width = _groups_of(parents, "reorder_pages")
     rows = groups * width
-    _need(table, "table", torch.int32)
-    _need(first, "first", torch.int32, (rows,))
-    _need(lengths, "lengths", torch.int32, (rows,))
-    if table.dim() != 2 or table.shape[0] != rows or pages.device != parents.device:
-        raise KernelError(f"reorder_pages: a table of shape {tuple(table.shape)} for {groups} groups of {width} rows on {pages.device}")
-    for n, bases, heads, count, row_bytes in _batches(pages.args):
-        _call("q6k_reorder_pages", _i(n), bases, heads, count, row_bytes, _ptr(table), _i(groups), _i(width), _i(table.shape[1]), _i(pages.page_size), _ptr(parents),
-              _ptr(first), _ptr(lengths), _stream())
+    _is(first, "first", torch.int32, (rows,))
+    _is(lengths, "lengths", torch.int32, (rows,))
+    if table.dim() != 2 or pages.device.index != device:
+        raise KernelError(f"reorder_pages: a table of shape {tuple(table.shape)} for {groups} groups of {width} rows, pages on {pages.device}")
+    _is(table, "table", torch.int32, (rows, table.shape[1]))
+    for n, *args in _batches(pages.args):
+        _call("q6k_reorder_pages", n, *args, table.data_ptr(), groups, width, table.shape[1], pages.page_size, parents.data_ptr(), first.data_ptr(), lengths.data_ptr(),
+              _stream_of(device))
 
 
 def reorder_slots(states, slots: torch.Tensor, parents: torch.Tensor) -> None:
     """The same for fixed-size states: row r's slot slots[r] takes over the slot of its parent, in every tensor of `states` (a
     SlotSet, or the tensors [slots, ...]).  slots: int32 [rows], no slot twice; a number outside the tensor: nothing is held."""
+    device = _here(("slots", slots), ("parents", parents))
     if not isinstance(states, SlotSet):
         states = SlotSet(states)
-    groups, width = _parents(parents, "reorder_slots")
-    _need(slots, "slots", torch.int32, (groups * width,))
-    if states.device != parents.device:
-        raise KernelError(f"reorder_slots: states on {states.device}, parents on {parents.device}")
-    for n, bases, count, nbytes in _batches(states.args):
-        _call("q6k_reorder_slots", _i(n), bases, count, nbytes, _ptr(slots), _i(groups), _i(width), _ptr(parents), _stream())
+    groups, width = _groups_of(parents, "reorder_slots")
+    _is(slots, "slots", torch.int32, (groups * width,))
+    if states.device.index != device:
+        raise KernelError(f"reorder_slots: states on {states.device}, the current device is cuda:{device}")
+    for n, *args in _batches(states.args):
+        _call("q6k_reorder_slots", n, *args, slots.data_ptr(), groups, width, parents.data_ptr(), _stream_of(device))

@@ -57,7 +57,7 @@ def matmul(a: torch.Tensor, w: torch.Tensor, rt, out: Optional[torch.Tensor] = N
     can sum split-K partial products itself, so the result may come as [slices, M, N] (a view of
     the device's scratch buffer: consume it before the next kernel that uses scratch)."""
     if isinstance(w, Int8Matrix):
-        return ops.linear_i8(a, w.q, w.scale, out=out, accumulate=accumulate)
+        return ops.linear_i8(a, w.q, w.scale, out=out, accumulate=accumulate, weights_are_old=True)
     if _tc(a, w, rt):
         if ops.gemv_preferred(a.shape[0], w.shape[0], w.shape[1]):       # a token or two: the matrix-vector kernel
             return ops.gemv(a, w, out=out, accumulate=accumulate)
@@ -75,7 +75,7 @@ def matmul(a: torch.Tensor, w: torch.Tensor, rt, out: Optional[torch.Tensor] = N
 def swiglu_matmul(a: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, rt, act=None) -> torch.Tensor:
     """y[r] = act(a[r] @ w_gate^T) * (a[r] @ w_up^T) in a's dtype; act None: silu."""
     if isinstance(w_gate, Int8Matrix):
-        return ops.linear_i8(a, w_gate.q, w_gate.scale, w2=w_up.q, w2_scale=w_up.scale, act=act)
+        return ops.linear_i8(a, w_gate.q, w_gate.scale, w2=w_up.q, w2_scale=w_up.scale, act=act, weights_are_old=True)
     if _tc(a, w_gate, rt):
         # the kernel for one or two tokens takes activations without a constant
         if not ops.act_has_param(act) and ops.gemv_preferred(a.shape[0], w_gate.shape[0], w_gate.shape[1]):
@@ -172,11 +172,13 @@ def _uniform_groups(groups: int, rows_per_group: int, bm: int, device):
     return _uniform[key]
 
 
-def pair_products(a: torch.Tensor, sel_e: torch.Tensor, per_row: int, w: "Int8Matrix", w_up: Optional["Int8Matrix"] = None, act=None) -> torch.Tensor:
+def pair_products(a: torch.Tensor, sel_e: torch.Tensor, per_row: int, w: "Int8Matrix", w_up: Optional["Int8Matrix"] = None, act=None,
+                  pairs_are_old: bool = False) -> torch.Tensor:
     """A step of few tokens: y[p] = a[p // per_row] @ w_e^T for the expert e of pair p, FP32 (or act of it, or the gated form with
-    w_up, in bfloat16), straight from the selection."""
+    w_up, in bfloat16), straight from the selection.  pairs_are_old: the kernel before this call did not make the selection."""
     more = {} if w_up is None else {"w2": w_up.q, "w2_scale": w_up.scale}
-    return ops.linear_i8(a, w.q, w.scale, act=act, pair_expert=sel_e.view(-1), pair_div=per_row, **more)
+    return ops.linear_i8(a, w.q, w.scale, act=act, pair_expert=sel_e.view(-1), pair_div=per_row,
+                         weights_are_old=pairs_are_old, **more)
 
 
 def batched_matmul(a: torch.Tensor, w: torch.Tensor, rt, rows_per_group: int, rounded: bool = False) -> torch.Tensor:

@@ -59,7 +59,7 @@ def plain_pairs(a, a_scale, g, w, w_scale, w2, w2_scale, act, out=None, accumula
     return y
 
 
-def plain_linear_i8(x, w, w_scale, out=None, accumulate=False, w2=None, w2_scale=None, act=None, pair_expert=None, pair_div=1):
+def plain_linear_i8(x, w, w_scale, out=None, accumulate=False, w2=None, w2_scale=None, act=None, pair_expert=None, pair_div=1, weights_are_old=False):
     q, s = plain_quantize_rows(x)
     if pair_expert is None:
         return plain_gemm_i8(q, s, w, w_scale, out, accumulate, w2, w2_scale, act)
