@@ -8,8 +8,10 @@
 // activation row and hands them to two instructions as if they were the layout's pieces; the four lanes that share a row cover
 // 64 contiguous bytes.  A block's eight warps split K in turns, a warp has all its loads of a turn in flight at once, and the
 // warps' sums meet in shared memory.
-// Rows that come in bfloat16 and hold few values in all are taken to 8 bits by every block for itself (by the rule of quantize.cuh),
-// while its first weights are on their way: one launch instead of two.
+// A single row that comes in bfloat16 is taken to 8 bits by every block for itself (by the rule of quantize.cuh), while its first
+// weights are on their way, where all blocks run at a time: 2,048 x 2,048 3.0 us where two launches take 3.8 (2.3 and 3.8 if the weights are
+// known to be old; 2,048 x 8,192 7.6 and 6.7, 6.4 and 6.7, and a launch less for the host); with more rows or more blocks the launch in front is
+// the shorter way (four rows 5.8 and 3.8, 2 x 8,192 x 2,048 18 and 10).
 #include "common.cuh"
 #include "gemm_i8.cuh"
 #include "quantize.cuh"
@@ -17,9 +19,6 @@
 namespace {
 
 constexpr int R8_WARPS = 8, R8_ROWS = 16;
-#ifndef I8_HERE
-#define I8_HERE 16384
-#endif
 
 __device__ __forceinline__ void r8_mma(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -28,19 +27,16 @@ __device__ __forceinline__ void r8_mma(int* c, uint32_t a0, uint32_t a1, uint32_
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Bytes between rows in shared memory: the eight lanes of two rows that are served at once read different banks.
-__host__ __device__ inline int r8_pitch(int K) { return (K + 127) / 128 * 128 + 64; }
-
 // grid: (blocks of 16 RB columns, 1 or pairs).  NB: blocks of 8 rows; RB: blocks of 16 columns; LOADS: 16-byte loads per lane and weight row in flight at once;
-// HERE: the rows are x in bfloat16, taken to 8 bits here.
+// HERE: the one row is x in bfloat16, taken to 8 bits here.
 template <bool DUAL, int NB, int RB, int LOADS, bool HERE>
 __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Args p) {
     pdl_launch();
     constexpr int MATS = DUAL ? 2 : 1, TURN = 64 * LOADS;
     __shared__ int meet[R8_WARPS][MATS * RB * NB * 4 * 32];
-    __shared__ unsigned most[HERE ? R8_ROWS : 1][R8_WARPS];
-    __shared__ float scale[HERE ? R8_ROWS : 1];
-    extern __shared__ __align__(16) int8_t rows8[];       // HERE: [rows, pitch]
+    __shared__ unsigned most[R8_WARPS];
+    extern __shared__ __align__(16) int8_t row8[];        // HERE: [K]
+    float scale = 0.0f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, pair = lane & 3;
     const int n0 = blockIdx.x * RB * 16, row0 = blockIdx.y, rows = p.pair_expert ? 1 : p.rows;
     if (!p.early) pdl_wait();
@@ -61,33 +57,26 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
             if (DUAL) wrow[1][rb][h] = p.w2 + r * p.K + pair * 16;
         }
     auto source = [&](int r) -> long long { return p.pair_expert ? r / p.pair_div : p.a_rows ? p.a_rows[r] : r; };
-    // every thread of the block once: the rows in 8 bits to shared memory
-    auto take_rows = [&] {
+    // every thread of the block once: the row in 8 bits to shared memory
+    auto take_row = [&] {
         if constexpr (HERE) {
-            for (int r = 0; r < rows; ++r) {
-                const __nv_bfloat16* from = p.x + source(row0 + r) * p.ldx;
-                unsigned m = 0;
-                for (int k = threadIdx.x * 8; k < p.K; k += R8_WARPS * 256) {
-                    Piece<__nv_bfloat16, 8> v;
-                    v.take(ld_after_wait(from + k));
-                    m = max(m, v.most());
-                }
-                m = __reduce_max_sync(0xffffffffu, m);
-                if (lane == 0) most[r][warp] = m;
+            unsigned m = 0;
+            for (int k = threadIdx.x * 8; k < p.K; k += R8_WARPS * 256) {
+                Piece<__nv_bfloat16, 8> v;
+                v.take(ld_after_wait(p.x + k));
+                m = max(m, v.most());
             }
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) most[warp] = m;
             __syncthreads();
-            for (int r = 0; r < rows; ++r) {
-                unsigned m = 0;
 #pragma unroll
-                for (int q = 0; q < R8_WARPS; ++q) m = max(m, most[r][q]);
-                const RowScale s = row_scale(m);
-                if (threadIdx.x == 0) scale[r] = s.scale;
-                const __nv_bfloat16* from = p.x + source(row0 + r) * p.ldx;
-                for (int k = threadIdx.x * 8; k < p.K; k += R8_WARPS * 256) {
-                    Piece<__nv_bfloat16, 8> v;
-                    v.take(ld_after_wait(from + k));
-                    v.store(rows8 + r * r8_pitch(p.K) + k, s.up);
-                }
+            for (int q = 0; q < R8_WARPS; ++q) m = max(m, most[q]);
+            const RowScale s = row_scale(m);
+            scale = s.scale;
+            for (int k = threadIdx.x * 8; k < p.K; k += R8_WARPS * 256) {
+                Piece<__nv_bfloat16, 8> v;
+                v.take(ld_after_wait(p.x + k));
+                v.store(row8 + k, s.up);
             }
             __syncthreads();
         }
@@ -112,11 +101,11 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
         if (first_turn) {
             first_turn = false;
             if (p.early) pdl_wait();
-            if constexpr (HERE) take_rows();
+            if constexpr (HERE) take_row();
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 live[nb] = nb * 8 + quad < rows;
-                if (HERE) xrow[nb] = rows8 + (live[nb] ? nb * 8 + quad : 0) * r8_pitch(p.K) + pair * 16;
+                if (HERE) xrow[nb] = row8 + pair * 16;
                 else xrow[nb] = p.a + source(live[nb] ? row0 + nb * 8 + quad : row0) * p.lda + pair * 16;
             }
         }
@@ -159,7 +148,7 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
             s += meet[q][idx];
             if (DUAL) s2 += meet[q][RB * NB * 4 * 32 + idx];
         }
-        const float xs = HERE ? scale[r] : p.a_scale[source(row0 + r)];
+        const float xs = HERE ? scale : p.a_scale[source(row0 + r)];
         const float v = (float)s * (xs * p.w_scale[first + n]);
         const float u = DUAL ? (float)s2 * (xs * p.w2_scale[first + n]) : 0.0f;
         i8_store<DUAL>(p, (long long)(row0 + r) * p.ldo + n, v, u);
@@ -168,9 +157,7 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
 
 template <bool DUAL, int NB, int RB, int LOADS>
 void launch(const I8Args& p, int pairs, cudaStream_t st) {
-    const dim3 grid((p.N + RB * 16 - 1) / (RB * 16), pairs);
-    if (p.x) q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS, true>, grid, R8_WARPS * 32, (p.pair_expert ? 1 : p.rows) * r8_pitch(p.K), st, p);
-    else q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS, false>, grid, R8_WARPS * 32, 0, st, p);
+    q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS, false>, dim3((p.N + RB * 16 - 1) / (RB * 16), pairs), R8_WARPS * 32, 0, st, p);
 }
 
 int launch_rows(const I8Args& p, cudaStream_t st) {
@@ -208,11 +195,11 @@ Q6K_API int q6k_gemm_i8(I8_OPERANDS, int a_total, void* gathered, float* gathere
     return q6k_gemm_i8_tc_launch(p, a_total, gathered, gathered_scale, tile, st);
 }
 
-// Values of bfloat16 rows up to which every block takes them to 8 bits itself.
-static bool taken_here(int T, int K, bool pairs) { return pairs ? K <= 8192 : (long long)T * K <= I8_HERE; }
-
-// Bytes of scratch that q6k_linear_i8 takes.
-Q6K_API long long q6k_linear_i8_scratch(int T, int K) { return (long long)T * K + 4LL * T; }
+// Bytes of scratch that q6k_linear_i8 takes for T rows of dtype code that lie on 16 bytes or do not, with a pair list or without; 0: the row is taken to 8
+// bits by the product's blocks, all of which run at a time.
+Q6K_API long long q6k_linear_i8_scratch(int T, int N, int K, int dtype, int aligned, int pairs) {
+    return T == 1 && !pairs && dtype == Q6K_BF16 && aligned && K <= 8192 && (N + 15) / 16 <= 2 * 148 ? 0 : (long long)T * K + 4LL * T;
+}
 
 // See ops.linear_i8: x of dtype code, T rows of pitch ldx; a, lda and a_scale of the operands are not looked at, and `early` says that the weights and
 // the pair list are older than the kernel before this call.  scratch: 16-byte aligned.
@@ -224,10 +211,15 @@ Q6K_API int q6k_linear_i8(const void* x, long long ldx, int T, int dtype, void* 
     Q6K_REQUIRE(!offsets && !a_rows && (pair_expert ? (rows + pair_div - 1) / pair_div <= T : rows == T), "linear_i8: %d rows of %d", rows, T);
     if (rows == 0) return 0;
     const bool few = pair_expert || rows <= R8_ROWS;
-    if (few && dtype == Q6K_BF16 && ldx % 8 == 0 && ((uintptr_t)x & 15) == 0 && taken_here(T, K, pair_expert != nullptr)) {
-        p.x = (const __nv_bfloat16*)x, p.ldx = ldx, p.early = early;
-        return launch_rows(p, st);
+    if (q6k_linear_i8_scratch(T, N, K, dtype, ((uintptr_t)x & 15) == 0, pair_expert != nullptr) == 0) {
+        p.x = (const __nv_bfloat16*)x, p.early = early;
+        const int blocks = (N + 15) / 16;
+        if (w2) q6k_launch_as(early != 0, gemm_i8_rows_kernel<true, 1, 1, 4, true>, blocks, R8_WARPS * 32, K, st, p);
+        else if (K > 4096) q6k_launch_as(early != 0, gemm_i8_rows_kernel<false, 1, 1, 8, true>, blocks, R8_WARPS * 32, K, st, p);
+        else q6k_launch_as(early != 0, gemm_i8_rows_kernel<false, 1, 1, 4, true>, blocks, R8_WARPS * 32, K, st, p);
+        return q6k_check_launch("linear_i8");
     }
+    Q6K_REQUIRE(scratch && ((uintptr_t)scratch & 15) == 0, "linear_i8: no scratch");
     if (int rc = q6k_quantize_rows_launch(x, ldx, T, K, dtype, scratch, (float*)p.a_scale, st)) return rc;
     return few ? launch_rows(p, st) : q6k_gemm_i8_tc_launch(p, T, nullptr, nullptr, 0, st);
 }

@@ -11,6 +11,8 @@
 //   others     epilogue: accumulators to registers, the two scales, the store
 // A gated product's tile holds 64 rows of the gate's matrix (lanes 0-63) and the same 64 of the other one (lanes 64-127); the
 // two warps that hold a column's two products exchange half of theirs through shared memory.
+// A product with fewer tiles than SMs and long rows cuts K over a cluster's CTAs (SPLIT): each leaves its 32-bit sums in its shared memory, and after a
+// barrier of the cluster every CTA adds up and finishes its share of the tile's rows.  The sums are integers, so the result is the same however K is cut.
 // Grouped products find their tiles from the groups' offsets in the kernel: no tile list is made.
 // Every wait on an mbarrier is bounded; a wait that runs out records a code that q6k_gemm_i8_status() returns, and the roles fall
 // through to the common exit.
@@ -33,6 +35,7 @@ struct TcArgs {
     I8Args p;
     int stages, n_x, n_y;              // tiles along N, and along the rows (dense)
     int w_once;                        // every weight tile is fetched once, or by few units side by side
+    int split;                         // SPLIT: CTAs of a cluster, which share a tile's K
 };
 
 // D: 32-bit integers, A and B signed 8-bit integers, both K-major, M rows, N = n.
@@ -118,7 +121,7 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, int t, int cols, const 
 
 __host__ __device__ constexpr int epilogue_warps(int bt) { return bt >= 64 ? 8 : 4; }
 
-template <int BT, int CTAS, bool DUAL>
+template <int BT, int CTAS, bool DUAL, bool SPLIT>
 __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
                                                                                     const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
                                                                                     const TcArgs a) {
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[MAX_STAGES]);
     const uint32_t acc_full0 = smem_u32(&bars[2 * MAX_STAGES]), acc_empty0 = smem_u32(&bars[2 * MAX_STAGES + 2]);
     const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
-    const int unit = blockIdx.x / CTAS, units = gridDim.x / CTAS;
+    const int per_unit = SPLIT ? a.split : CTAS, unit = blockIdx.x / per_unit, units = gridDim.x / per_unit;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
@@ -184,15 +187,18 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     pdl_launch();                                        // this block holds its tensor memory: a successor may come
-    const int total = a.n_x * (p.offsets ? starts[p.groups] : a.n_y), kbs = (p.K + BK - 1) / BK;
+    const int total = a.n_x * (p.offsets ? starts[p.groups] : a.n_y), kb_all = (p.K + BK - 1) / BK;
+    // the k-blocks of this CTA: kb0 .. kb0 + kbs - 1 (SPLIT: one tile for each cluster, and every slice has some)
+    const int slice = SPLIT ? (int)cluster_rank() : 0, slice_kbs = SPLIT ? (kb_all + a.split - 1) / a.split : kb_all;
+    const int kb0 = slice * slice_kbs, kbs = min(slice_kbs, kb_all - kb0);
 
     if (warp == 0) {
         if (elect_one()) {
             const uint64_t once = l2_evict_first_policy();
             auto load_w = [&](uint32_t st, uint32_t fb, int i, int wy, int n) {
                 if (rank == 0) mbar_expect_tx(fb, CTAS * W_BYTES + n * BK);
-                load<CTAS>(st, &tm_w, i * BK, wy, fb, a.w_once, once);
-                if (DUAL) load<CTAS>(st + W_BYTES / 2, &tm_w2, i * BK, wy, fb, a.w_once, once);
+                load<CTAS>(st, &tm_w, (kb0 + i) * BK, wy, fb, a.w_once, once);
+                if (DUAL) load<CTAS>(st + W_BYTES / 2, &tm_w2, (kb0 + i) * BK, wy, fb, a.w_once, once);
             };
             int pre = 0;                                 // k-blocks whose weights went out before the wait (with nothing to wait for, the first rows would queue behind them)
             for (int t = unit; p.early && t < total && pre < stages; t += units) {
@@ -218,9 +224,9 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
                         }
                         load_w(st, fb, i, wy, tl.n);
                     }
-                    if (tl.n == BT) load<CTAS>(st + W_BYTES, &tm_a, i * BK, ay, fb, false, once);
+                    if (tl.n == BT) load<CTAS>(st + W_BYTES, &tm_a, (kb0 + i) * BK, ay, fb, false, once);
                     else
-                        for (int c = 0; c < tl.n / CTAS; c += 32) load<CTAS>(st + W_BYTES + c * BK, &tm_a32, i * BK, ay + c, fb, false, once);
+                        for (int c = 0; c < tl.n / CTAS; c += 32) load<CTAS>(st + W_BYTES + c * BK, &tm_a32, (kb0 + i) * BK, ay + c, fb, false, once);
                     if (++s == stages) s = 0, st = ring, phase ^= 1;
                     else st += STAGE_BYTES;
                 }
@@ -298,7 +304,17 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
                 if (lane == 0) arrive_leader<CTAS>(acc_empty0 + 8 * buf);
             };
             if (end <= 0) release();
-            if constexpr (DUAL) {
+            if constexpr (SPLIT) {                       // the sums of this slice, row by row, where the ring was (every MMA has read it)
+#pragma unroll 1
+                for (int c0 = 0; ok && c0 < end; c0 += 16) {
+                    float v[16];
+                    tmem_ld16_issue(from + c0, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((part * span + c0 + j) * WM + quarter * 32 + lane) * 4), "f"(v[j]) : "memory");
+                }
+            } else if constexpr (DUAL) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < end; c0 += 32, ++turn) {
                     float v[16], u[16];                  // 32-bit integers until they are scaled
@@ -387,6 +403,36 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (SPLIT) {
+        cluster_sync();                                  // every slice's sums are there
+        const Tile tl = tile_of<BT, CTAS>(a, unit, COLS, starts);
+        const int rows = min(tl.row_end - tl.row0, BT), share = (rows + a.split - 1) / a.split, r0 = slice * share, r1 = min(rows, r0 + share);
+        for (int i = r0 * (COLS / 4) + threadIdx.x; i < r1 * (COLS / 4); i += blockDim.x) {
+            const int r = i / (COLS / 4), c = i % (COLS / 4) * 4;
+            int s[4] = {}, s2[4] = {};
+            for (int q = 0; q < a.split; ++q) {
+                int v[4];
+                uint32_t at;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ring + (r * WM + c) * 4), "r"(q));
+                asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] += v[j];
+                if (DUAL) {
+                    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at + COLS * 4) : "memory");
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s2[j] += v[j];
+                }
+            }
+            const float xs = p.a_scale[tl.row0 + r];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int n = tl.n0 + c + j;
+                if (n < p.N)
+                    i8_store<DUAL>(p, (long long)(tl.row0 + r) * p.ldo + n, (float)s[j] * (xs * p.w_scale[n]), DUAL ? (float)s2[j] * (xs * p.w2_scale[n]) : 0.0f);
+            }
+        }
+        cluster_sync();                                  // nobody leaves while others read its sums
+    }
     if constexpr (CTAS == 2) cluster_sync();             // the peer has no MMA, copy or arrival of ours in flight
     if (warp == 1) {
         tc_fence_after();
@@ -438,7 +484,7 @@ int sm_count() {
     return n;
 }
 
-template <int BT, int CTAS, bool DUAL>
+template <int BT, int CTAS, bool DUAL, bool SPLIT = false>
 int launch(const TcArgs& args, int a_total, cudaStream_t st) {
     TcArgs t = args;
     const I8Args& p = t.p;
@@ -462,17 +508,18 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
     const size_t smem = (size_t)t.stages * stage + extra + 1024;
     static bool configured = false;
     if (!configured) {
-        if (cudaFuncSetAttribute(gemm_i8_tc_kernel<BT, CTAS, DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess)
+        if (cudaFuncSetAttribute(gemm_i8_tc_kernel<BT, CTAS, DUAL, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess)
             return q6k_check_launch("gemm_i8: shared memory attribute");
         configured = true;
     }
-    const int units = sm_count() / CTAS;
+    const int units = sm_count() / CTAS, cluster = SPLIT ? t.split : CTAS;
+    Q6K_REQUIRE(!SPLIT || total * cluster <= 0x7fffffff, "gemm_i8: %lld tiles of %d slices", total, cluster);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CTAS * (unsigned)(total < units ? total : units)), cfg.blockDim = dim3(64 + 32 * EW), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.gridDim = dim3(cluster * (unsigned)(SPLIT || total < units ? total : units)), cfg.blockDim = dim3(64 + 32 * EW), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr[2];
-    if (CTAS == 2) {
+    if (cluster > 1) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = CTAS, attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster, attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
     if (i8_overlaps(p)) {
@@ -481,28 +528,37 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
         ++cfg.numAttrs;
     }
     cfg.attrs = attr;
-    cudaLaunchKernelEx(&cfg, gemm_i8_tc_kernel<BT, CTAS, DUAL>, tw, tw2, ta, ta32, t);
+    cudaLaunchKernelEx(&cfg, gemm_i8_tc_kernel<BT, CTAS, DUAL, SPLIT>, tw, tw2, ta, ta32, t);
     return q6k_check_launch("gemm_i8");
 }
 
 // Rows of a tile (negative: a pair of CTAs).  A unit's time for one tile of K = 2,048, in tenths of a microsecond, measured over many tiles (8,192 x 2
 // columns): a wide tile re-reads less and feeds the tensor cores better, a narrow one leaves fewer units idle in the last round.  With the least
-// rounds x time, 1,522 rows x (2 x 8,192), K 2,048 take 41.1 us on pairs of 192 (42.2 of 256; 53.7 with single CTAs of 128), 256 rows x 2,048 take
+// rounds x time, 1,522 rows x (2 x 8,192), K 2,048 take 40.8 us on pairs of 256 (42.6 of 192; 60.3 with single CTAs of 128), 256 rows x 2,048 take
 // 6.6 us on tiles of 32 (7.2 of 128, 11.1 on pairs), 64 rows x (2 x 8,192) 9.7 on 64 (12.8 on 32), all in a graph with weights from HBM.
 // Grouped rows: the experts' shares are known on the device only, so half as much again as an even share.
-int choose_tile(const I8Args& p, bool dual) {
+// split: CTAs that share a tile's K, where that takes less time: a slice's share of it and two microseconds for the sums to meet (2,048 columns, K 8,192,
+// 32 rows: 16.8 us in 16 CTAs, 10.3 in four slices; K 2,048: 7.0 and 7.0, in two 8.4).
+int choose_tile(const I8Args& p, bool dual, int* split) {
+    *split = 1;
     if (p.offsets) {
         const int share = p.rows / p.groups + p.rows / p.groups / 2;
         return share <= 32 ? 32 : share <= 64 ? 64 : 128;
     }
-    static const int tiles[][2] = {{32, 35}, {64, 38}, {128, 47}, {256, 76}, {-192, 52}, {-256, 69}};
+    static const int tiles[][2] = {{32, 35}, {64, 38}, {128, 47}, {256, 76}, {-192, 56}, {-256, 64}};
     long long best = -1;
     int pick = 0;
     for (auto& t : tiles) {
         const int bt = t[0] < 0 ? -t[0] : t[0], ctas = t[0] < 0 ? 2 : 1, cols = ctas * (dual ? WM / 2 : WM);
         const long long units = sm_count() / ctas, count = (long long)((p.N + cols - 1) / cols) * ((p.rows + bt - 1) / bt);
-        const long long cost = (count + units - 1) / units * t[1];
-        if (best < 0 || cost < best) best = cost, pick = t[0];
+        const int kbs = (p.K + BK - 1) / BK;
+        const long long cost = (count + units - 1) / units * t[1] * kbs;                  // in units of a sixteenth of a tenth of a microsecond
+        if (best < 0 || cost < best) best = cost, pick = t[0], *split = 1;
+        // clusters whose CTAs all run at a time: 96 in eights, 128 in fours and twos (of 148 SMs; 16 clusters of eight took two rounds)
+        for (int s = 2; ctas == 1 && bt <= 128 && s <= 8 && count * s <= (s == 8 ? 96 : 128) && (s - 1) * ((kbs + s - 1) / s) < kbs; s *= 2) {
+            const long long cut = (long long)t[1] * ((kbs + s - 1) / s) + 16 * 20;
+            if (cut < best) best = cut, pick = t[0], *split = s;
+        }
     }
     return pick;
 }
@@ -516,7 +572,7 @@ Q6K_API int q6k_gemm_i8_status() {
 }
 
 // More than a few rows, or groups.  gathered, gathered_scale (with a_rows): int8 [rows, K] and FP32 [rows] of scratch.  tile: rows of a tile, negative for
-// pairs of CTAs (0: chosen here).
+// pairs of CTAs (0: chosen here), with 1000 s added for s slices of K.
 int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st) {
     TcArgs t{p};
     if (p.rows == 0) return 0;
@@ -530,7 +586,17 @@ int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, float* g
     }
     Q6K_REQUIRE(a_total >= p.rows, "gemm_i8: %d rows of %d", p.rows, a_total);
     const bool dual = p.w2 != nullptr;
-    if (tile == 0) tile = choose_tile(t.p, dual);
+    t.split = 1;
+    if (tile == 0) tile = choose_tile(t.p, dual, &t.split);
+    else if (tile > 1000) t.split = tile / 1000, tile %= 1000;
+    if (t.split > 1) {
+        const int kbs = (p.K + BK - 1) / BK;
+        Q6K_REQUIRE(!p.offsets && t.split <= 8 && (t.split - 1) * ((kbs + t.split - 1) / t.split) < kbs, "gemm_i8: K=%d in %d slices", p.K, t.split);
+        if (tile == 32) return dual ? launch<32, 1, true, true>(t, a_total, st) : launch<32, 1, false, true>(t, a_total, st);
+        if (tile == 64) return dual ? launch<64, 1, true, true>(t, a_total, st) : launch<64, 1, false, true>(t, a_total, st);
+        if (tile == 128) return dual ? launch<128, 1, true, true>(t, a_total, st) : launch<128, 1, false, true>(t, a_total, st);
+        return q6k_fail("gemm_i8: tiles of %d rows in slices", tile);
+    }
 #define GO(T_, BT_, CTAS_) \
     case T_: return dual ? launch<BT_, CTAS_, true>(t, a_total, st) : launch<BT_, CTAS_, false>(t, a_total, st)
     switch (tile) {

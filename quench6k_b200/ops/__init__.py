@@ -2182,6 +2182,13 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     return out
 
 
+@functools.lru_cache(maxsize=1024)          # a question about sizes: asked of the library once
+def _linear_i8_scratch(T: int, N: int, K: int, code: int, aligned: bool, pairs: bool) -> int:
+    lib = library()
+    lib.q6k_linear_i8_scratch.restype = ctypes.c_longlong
+    return lib.q6k_linear_i8_scratch(_i(T), _i(N), _i(K), _i(code), _i(aligned), _i(pairs))
+
+
 def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool = False,
               w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None, pair_expert: Optional[torch.Tensor] = None,
               pair_div: int = 1, weights_are_old: bool = False) -> torch.Tensor:
@@ -2204,9 +2211,10 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Opti
             raise KernelError(f"linear_i8: {pairs} pairs (at most 65535), {pair_div} for each of {T} rows")
     rows = T if pair_expert is None else pairs
     groups, N, epi, out = _i8_product(w, w_scale, w2, w2_scale, K, pair_expert is not None, accumulate, act, out, rows, "linear_i8")
-    scratch = torch.empty(T * K + 4 * T, dtype=torch.uint8, device=x.device)
-    _call("q6k_linear_i8", x.data_ptr(), pitch, T, code, scratch.data_ptr(), 0, K, 0, rows, w.data_ptr(), w_scale.data_ptr(), _data(w2), _data(w2_scale), N, K, 0, 0,
-          groups, _data(pair_expert), pair_div, out.data_ptr(), N, epi, _act_param(act), weights_are_old, _stream_of(device), launches=2 if rows else 0)
+    nbytes = _linear_i8_scratch(T, N, K, code, x.data_ptr() % 16 == 0, pair_expert is not None)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _call("q6k_linear_i8", x.data_ptr(), pitch, T, code, _data(scratch), 0, K, 0, rows, w.data_ptr(), w_scale.data_ptr(), _data(w2), _data(w2_scale), N, K, 0, 0,
+          groups, _data(pair_expert), pair_div, out.data_ptr(), N, epi, _act_param(act), weights_are_old, _stream_of(device), launches=0 if rows == 0 else 1 if scratch is None else 2)
     return out
 
 

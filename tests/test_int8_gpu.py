@@ -114,7 +114,8 @@ STORED = 3 * HALF * (1 + 1e-6)
 GATED = BF16_HALF + (3 * 201 + 3 + 10 + 201) * HALF
 
 SHAPES = [(1, 1, 16), (1, 2048, 2048), (2, 100, 48), (3, 17, 1024), (8, 64, 64), (9, 4097, 80), (16, 129, 4096), (17, 128, 128), (32, 1000, 2048), (33, 257, 272),
-          (64, 384, 512), (100, 640, 1040), (129, 300, 144), (200, 129, 8192), (257, 512, 2064), (300, 7, 16), (1000, 1024, 256)]
+          (64, 384, 512), (100, 640, 1040), (129, 300, 144), (200, 129, 8192), (257, 512, 2064), (300, 7, 16), (1000, 1024, 256),
+          (17, 512, 10240), (100, 200, 8208), (48, 2048, 8192), (250, 1100, 4112), (130, 90, 1168)]      # few tiles and long rows: K in slices
 
 
 @pytest.mark.parametrize("rows,n,k", SHAPES)
@@ -126,7 +127,7 @@ def test_product(rows, n, k):
     near(y, product64(a, s, w, t), STORED)
 
 
-@pytest.mark.parametrize("rows,n,k", [(1, 300, 512), (12, 129, 64), (40, 256, 2048), (300, 520, 528)])
+@pytest.mark.parametrize("rows,n,k", [(1, 300, 512), (12, 129, 64), (40, 256, 2048), (300, 520, 528), (30, 300, 8192)])
 def test_product_added(rows, n, k):
     from quench6k_b200 import ops
     a, s, ((w, t),) = operands(rows, rows, n, k)
@@ -139,7 +140,7 @@ def test_product_added(rows, n, k):
 
 
 @pytest.mark.parametrize("act", [None, "gelu_tanh", "relu2", ("clamped", 7.0)])
-@pytest.mark.parametrize("rows,n,k", [(1, 512, 2048), (16, 130, 272), (70, 129, 512), (600, 300, 1040), (1200, 1024, 256)])
+@pytest.mark.parametrize("rows,n,k", [(1, 512, 2048), (16, 130, 272), (70, 129, 512), (600, 300, 1040), (1200, 1024, 256), (40, 250, 8192), (200, 70, 4112)])
 def test_gated_product(rows, n, k, act):
     from quench6k_b200 import ops
     a, s, ((w, t), (w2, t2)) = operands(rows * 3 + n, rows, n, k, mats=2)
@@ -153,7 +154,7 @@ def test_gated_product(rows, n, k, act):
 
 
 @pytest.mark.parametrize("act", ["silu", "relu2"])
-@pytest.mark.parametrize("rows,n,k", [(5, 64, 128), (150, 300, 256)])
+@pytest.mark.parametrize("rows,n,k", [(5, 64, 128), (150, 300, 256), (20, 100, 6144)])
 def test_activated_product(rows, n, k, act):
     from quench6k_b200 import ops
     a, s, ((w, t),) = operands(rows, rows, n, k)
@@ -217,6 +218,23 @@ def test_product_pair_by_pair(tokens, top, n, k, gated, dtype):
             near(out[i:i + 1], gated64(y, product64(q[row], s[row], mats[1][0][g], mats[1][1][g] * 0.02), None), GATED, 1e-30)
         else:
             near(out[i:i + 1], y, STORED)
+
+
+@pytest.mark.parametrize("old", [False, True])
+@pytest.mark.parametrize("k", [16, 2032, 4096, 8192])
+@pytest.mark.parametrize("bad", [False, True])
+def test_one_row_taken_to_8_bits_inside_the_product(k, bad, old):
+    """The same numbers as in two calls, for rows of zeros and rows that are not finite too."""
+    from quench6k_b200 import ops
+    _, _, ((w, t), (w2, t2)) = operands(k, 1, 333, k, mats=2)
+    w, t, w2, t2 = w.cuda(), t.cuda() * 0.01, w2.cuda(), t2.cuda() * 0.01
+    rows = [rows_of(3, 1, k, torch.bfloat16)[0].contiguous(), torch.zeros(1, k, dtype=torch.bfloat16, device="cuda")]
+    if bad:
+        rows[0][0, k - 1], rows[1][0, 0] = float("nan"), -float("inf")
+    for x in rows:
+        q, s = ops.quantize_rows(x)
+        for more in ({}, {"w2": w2, "w2_scale": t2}, {"act": "relu2"}):
+            assert torch.equal(ops.linear_i8(x, w, t, weights_are_old=old, **more).nan_to_num(7.0), ops.gemm_i8(q, s, w, t, **more).nan_to_num(7.0))
 
 
 @pytest.mark.parametrize("rows", [1, 4, 7, 16, 17, 40, 130])
