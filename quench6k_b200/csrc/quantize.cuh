@@ -15,7 +15,7 @@ __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v
 // N neighbouring values at p as they are stored; N > 1: 16 bytes at once.
 template <typename T, int N>
 struct Piece {
-    T v[N];
+    alignas(N * sizeof(T)) T v[N];
     __device__ __forceinline__ void take(const uint4& bytes) {
         static_assert(N * sizeof(T) == 16, "16 bytes");
         *(uint4*)v = bytes;
@@ -26,17 +26,35 @@ struct Piece {
     }
     __device__ __forceinline__ unsigned most() const {
         unsigned m = 0;
+        if constexpr (sizeof(T) == 2 && N > 1) {                               // two values to an instruction: their upper halves are all there is
+            const unsigned* w = (const unsigned*)v;
 #pragma unroll
-        for (int i = 0; i < N; ++i) m = max(m, abs_bits(to_f32(v[i])));
-        return m;
+            for (int i = 0; i < N / 2; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            return max(m & 0xffff0000u, m << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) m = max(m, abs_bits(to_f32(v[i])));
+            return m;
+        }
     }
-    __device__ __forceinline__ void store(int8_t* q, float u) const {          // u = 0: zeros, whatever the values are
-        union { int8_t b[N]; unsigned w[(N + 3) / 4]; } o;
+    // up = 0: zeros, whatever the values are.  A product below 2^22 plus 1.5 x 2^23 is rounded to a whole number, ties to even, whose lowest byte is the
+    // entry: an addition for each value and three byte selections for four, where conversions run at a quarter of the rate (8,192 rows of 8,192: 37 us
+    // with them, 31 without).
+    __device__ __forceinline__ void store(int8_t* q, float up) const {
+        unsigned w[(N + 3) / 4] = {};
+        if (up != 0.0f) {
+            unsigned b[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) o.b[i] = u == 0.0f ? (int8_t)0 : (int8_t)__float2int_rn(to_f32(v[i]) * u);
-        if constexpr (N == 1) *q = o.b[0];
-        else if constexpr (N == 4) *(unsigned*)q = o.w[0];
-        else *(uint2*)q = make_uint2(o.w[0], o.w[1]);
+            for (int i = 0; i < N; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(to_f32(v[i]), up), 12582912.0f));
+            if constexpr (N == 1) w[0] = b[0];
+            else {
+#pragma unroll
+                for (int i = 0; i < N; i += 4) w[i / 4] = __byte_perm(__byte_perm(b[i], b[i + 1], 0x0040), __byte_perm(b[i + 2], b[i + 3], 0x0040), 0x5410);
+            }
+        }
+        if constexpr (N == 1) *q = (int8_t)w[0];
+        else if constexpr (N == 4) *(unsigned*)q = w[0];
+        else *(uint2*)q = make_uint2(w[0], w[1]);
     }
 };
 
