@@ -15,7 +15,7 @@ namespace {
 
 constexpr int SEL_THREADS = 256, SEL_MAX_COUNT = 128, SEL_MAX_WIDTH = 32;
 constexpr int SEL_EACH = 32, SEL_TILE = SEL_THREADS * SEL_EACH;
-constexpr int MERGE_THREADS = 512, MERGE_WARPS = MERGE_THREADS / 32;
+constexpr int MERGE_THREADS = 512, MERGE_WARPS = MERGE_THREADS / 32, MERGE_HELD = 4;
 constexpr int SEL_WARPS = SEL_THREADS / 32, SEL_POOL = 1024, SEL_TILES = 8;       // keys that a pool holds; the most tiles of a part
 constexpr int SEL_PARTS = 4;       // parts to an SM that a long batch is cut into (8: 29 us where 4 take 25, 128 rows of 151,936 logits: more parts leave more to merge)
 constexpr float LOG2E = 1.4426950408889634f;
@@ -46,10 +46,29 @@ __device__ __forceinline__ int block_count(int v, int* red) {
 }
 
 // The best `count` of many keys without sorting them: a number that at least `count` of them reach and few others do.  Every thread brings the largest
-// of the keys that it holds; the count-th largest of those is found from its highest bit down, and no further than until few more reach it than are
-// wanted.  0: fewer than `count` threads hold any.
-__device__ __forceinline__ unsigned block_threshold(unsigned mine, int count) {
+// of the keys that it holds.  Few wanted: the first warp's lanes take the largest of THREADS / 32 of those each, and the count-th largest of the 32 is taken out
+// by one maximum after the other.  Otherwise the count-th largest of all threads' keys is found from its highest bit down, a barrier for each bit, and no further
+// than until few more reach it than are wanted (eight wanted of 512 keys: 1.1 us that way, 0.5 the other; with sixteen wanted more keys are let through than the barriers cost).
+// 0: fewer than `count` of those hold any key.  slot: THREADS words of shared memory.
+template <int THREADS>
+__device__ __forceinline__ unsigned block_threshold(unsigned mine, int count, unsigned* slot) {
     unsigned t = 0;
+    if (count <= 12) {
+        slot[threadIdx.x] = mine;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            unsigned k = 0;
+#pragma unroll
+            for (int i = 0; i < THREADS / 32; ++i) k = max(k, slot[i * 32 + threadIdx.x]);
+            for (int i = 0; i < count; ++i) {
+                t = __reduce_max_sync(0xffffffffu, k);
+                if ((int)threadIdx.x == __ffs(__ballot_sync(0xffffffffu, k == t)) - 1) k = 0;
+            }
+            if (threadIdx.x == 0) slot[0] = t;
+        }
+        __syncthreads();
+        return slot[0];
+    }
     for (int bit = 31; bit >= 0; --bit) {
         const unsigned trial = t | (1u << bit);
         const int c = __syncthreads_count(mine >= trial);
@@ -71,7 +90,8 @@ template <bool WIDE>
 __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* logits, int V, int tiles, int count, float* best, int* at, PartHead* heads) {
     pdl_enter();
     __shared__ int red[SEL_WARPS];
-    __shared__ float redf[32], redm[SEL_WARPS];
+    __shared__ PartHead of_warp[SEL_WARPS];
+    __shared__ unsigned slots[SEL_THREADS];
     __shared__ unsigned key[SEL_POOL];
     __shared__ int place[SEL_POOL];
     __shared__ float piece_most[SEL_TILES][SEL_THREADS];
@@ -125,17 +145,25 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
                 if (!(v[j] == -INFINITY)) sum = NAN;         // nothing but NaNs
         }
     }
-    float block_most = warp_max(most);
-    if (lane == 0) redm[warp] = block_most;
-    const unsigned low = block_threshold(finite_key(most), count);
+    const float warp_most = warp_max(most);
+    if (most > -INFINITY) sum *= ex2_approx((most - warp_most) * LOG2E);
+    sum = warp_sum(sum);
+    if (lane == 0) of_warp[warp] = PartHead{warp_most, sum};
+    const unsigned low = block_threshold<SEL_THREADS>(finite_key(most), count, slots);
     const float reach = low != 0 ? key_value(low) : -FLT_MAX;
+    if (threadIdx.x == 0) {
+        PartHead h = of_warp[0];
 #pragma unroll
-    for (int w = 0; w < SEL_WARPS; ++w) block_most = fmaxf(block_most, redm[w]);
+        for (int w = 1; w < SEL_WARPS; ++w) h.most = fmaxf(h.most, of_warp[w].most);
+        h.sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < SEL_WARPS; ++w)
+            if (of_warp[w].sum != 0.0f) h.sum += of_warp[w].sum * ex2_approx((of_warp[w].most - h.most) * LOG2E);
+        heads[slot] = h;
+    }
     for (int t = 0; t < tiles && lo + t * SEL_TILE < hi; ++t)
         if (piece_most[t][threadIdx.x] >= reach && most < INFINITY) pieces[atomicAdd(&listed, 1)] = (unsigned short)(t * SEL_THREADS + threadIdx.x);
-    if (most > -INFINITY) sum *= ex2_approx((most - block_most) * LOG2E);
-    sum = block_sum(sum, redf);
-    if (threadIdx.x == 0) heads[slot] = PartHead{block_most, sum};
+    __syncthreads();
     for (int i = warp; i < listed; i += SEL_WARPS) {
         const int t = pieces[i] / SEL_THREADS, p = lo + t * SEL_TILE + where(pieces[i] % SEL_THREADS, lane);
         const float v = p < hi ? row[p] : -INFINITY;
@@ -153,6 +181,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
             int rank = 0;
             const unsigned k = key[i];
             const int p = place[i];
+#pragma unroll 8
             for (int j = 0; j < found; ++j) rank += key[j] > k || (key[j] == k && place[j] < p);
             if (rank < count) best[rank] = key_value(k), at[rank] = p;
         }
@@ -192,13 +221,23 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(const float* 
     pdl_enter();
     __shared__ double base[SEL_MAX_WIDTH], row_most[SEL_MAX_WIDTH];      // the beam's score less the logarithm of its row's sum over the row's maximum
     __shared__ bool dead[SEL_MAX_WIDTH];
-    __shared__ int red[MERGE_THREADS / 32];
+    __shared__ int red[MERGE_WARPS];
+    __shared__ unsigned slots[MERGE_THREADS];
     __shared__ unsigned long long key[SEL_POOL];
     __shared__ int place[SEL_POOL];
     __shared__ int taken;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t row0 = (size_t)blockIdx.x * width;
     heads += row0 * parts, best += row0 * parts * count, at += row0 * parts * count, scores += row0;
+    const int per_row = parts * count, all = width * per_row;
+    // a thread's first candidates are asked for before the rows' sums are made, and kept
+    int held_at[MERGE_HELD];
+    float held_best[MERGE_HELD];
+#pragma unroll
+    for (int h = 0; h < MERGE_HELD; ++h) {
+        const int i = h * MERGE_THREADS + threadIdx.x;
+        held_at[h] = i < all ? at[i] : -1, held_best[h] = i < all ? best[i] : 0.0f;
+    }
     for (int b = warp; b < width; b += MERGE_WARPS) {
         const float score = scores[b];
         float most = -INFINITY;
@@ -221,21 +260,23 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(const float* 
     }
     if (threadIdx.x == 0) taken = 0;
     __syncthreads();
-    const int per_row = parts * count, all = width * per_row;
     const float inverse = 1.0f / (float)per_row;
+    auto one = [&](int i, int token, float value, auto&& f) {
+        int b = (int)((float)i * inverse);
+        b -= b * per_row > i, b += (b + 1) * per_row <= i;
+        if (token >= 0 && !dead[b]) f(score_key(base[b] + ((double)value - row_most[b])), b * V + token);
+    };
     auto each = [&](auto&& f) {                              // every candidate; the rows are spread over all threads
-        for (int i = threadIdx.x; i < all; i += MERGE_THREADS) {
-            const int token = at[i];
-            int b = (int)((float)i * inverse);
-            b -= b * per_row > i, b += (b + 1) * per_row <= i;
-            if (token >= 0 && !dead[b]) f(score_key(base[b] + ((double)best[i] - row_most[b])), b * V + token);
-        }
+#pragma unroll
+        for (int h = 0; h < MERGE_HELD; ++h) one(h * MERGE_THREADS + threadIdx.x, held_at[h], held_best[h], f);
+#pragma unroll 4
+        for (int i = MERGE_HELD * MERGE_THREADS + threadIdx.x; i < all; i += MERGE_THREADS) one(i, at[i], best[i], f);
     };
     unsigned long long mine = 0;
     int c = 0;
     each([&](unsigned long long k, int) { mine = k > mine ? k : mine, ++c; });
     const int want = min(count, block_count<MERGE_WARPS>(c, red));
-    const unsigned long long reach = (unsigned long long)block_threshold((unsigned)(mine >> 32), count) << 32;
+    const unsigned long long reach = (unsigned long long)block_threshold<MERGE_THREADS>((unsigned)(mine >> 32), count, slots) << 32;
     auto take = [&](unsigned long long k, int w) {
         const int to = atomicAdd(&taken, 1);
         if (to < SEL_POOL) key[to] = k, place[to] = w;
@@ -274,6 +315,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(const float* 
         int rank = 0;
         const unsigned long long u = key[i];
         const int w = place[i];
+#pragma unroll 8
         for (int j = 0; j < found; ++j) rank += key[j] > u || (key[j] == u && place[j] < w);
         if (rank >= want) continue;
         out_score[rank] = (float)__longlong_as_double((long long)((u >> 63) ? u & ~(1ull << 63) : ~u));
