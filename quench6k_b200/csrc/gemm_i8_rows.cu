@@ -43,7 +43,10 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
     int g = 0;
     if (p.pair_expert) {
         g = p.pair_expert[row0];
-        if ((unsigned)g >= (unsigned)p.groups) return;
+        if ((unsigned)g >= (unsigned)p.groups) {
+            if (p.early) pdl_wait();                      // a block that ends has waited too: who waits for this kernel counts on it
+            return;
+        }
     }
     const uint64_t once = l2_evict_first_policy();
     const long long first = (long long)g * p.N;
@@ -183,16 +186,16 @@ int launch_rows(const I8Args& p, cudaStream_t st) {
 }  // namespace
 
 int q6k_quantize_rows_launch(const void* x, long long ldx, int R, int K, int dtype, void* q, float* scale, cudaStream_t st);
-int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st);
+int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, cudaStream_t st);
 
-// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered, gathered_scale: int8 [rows, K] and FP32 [rows] of scratch, where a_rows comes with
-// more than 16 rows or with groups.  tile: see q6k_gemm_i8_tc_launch (0 but for measurements).
-Q6K_API int q6k_gemm_i8(I8_OPERANDS, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st) {
+// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered: rows * (K + 4) bytes of scratch, where a_rows comes with more than 16 rows or with
+// groups.
+Q6K_API int q6k_gemm_i8(I8_OPERANDS, int a_total, void* gathered, cudaStream_t st) {
     I8Args p;
     if (int rc = i8_args(&p, "gemm_i8", I8_NAMES)) return rc;
     Q6K_REQUIRE(!pair_expert, "gemm_i8: pairs come with rows that are not in 8 bits");
-    if (rows <= R8_ROWS && !offsets && tile == 0) return launch_rows(p, st);
-    return q6k_gemm_i8_tc_launch(p, a_total, gathered, gathered_scale, tile, st);
+    if (rows <= R8_ROWS && !offsets) return launch_rows(p, st);
+    return q6k_gemm_i8_tc_launch(p, a_total, gathered, st);
 }
 
 // Bytes of scratch that q6k_linear_i8 takes for T rows of dtype code that lie on 16 bytes or do not, with a pair list or without; 0: the row is taken to 8
@@ -221,5 +224,5 @@ Q6K_API int q6k_linear_i8(const void* x, long long ldx, int T, int dtype, void* 
     }
     Q6K_REQUIRE(scratch && ((uintptr_t)scratch & 15) == 0, "linear_i8: no scratch");
     if (int rc = q6k_quantize_rows_launch(x, ldx, T, K, dtype, scratch, (float*)p.a_scale, st)) return rc;
-    return few ? launch_rows(p, st) : q6k_gemm_i8_tc_launch(p, T, nullptr, nullptr, 0, st);
+    return few ? launch_rows(p, st) : q6k_gemm_i8_tc_launch(p, T, nullptr, st);
 }

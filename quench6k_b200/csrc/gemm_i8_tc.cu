@@ -16,6 +16,8 @@
 // Grouped products find their tiles from the groups' offsets in the kernel: no tile list is made.
 // Every wait on an mbarrier is bounded; a wait that runs out records a code that q6k_gemm_i8_status() returns, and the roles fall
 // through to the common exit.
+#include <atomic>
+
 #include "common.cuh"
 #include "gemm_i8.cuh"
 #include "tma.cuh"
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
                         float* o = (float*)p.out + at;
 #pragma unroll
                         for (int j = 0; j < 16; ++j, o += p.ldo)
-                            if (j < rows) atomicAdd(o, v[j]);
+                            if (j < rows) atomicAdd(o, v[j]);      // (a sum below 1.2e-38 may become 0)
                     } else if (rows >= 16) {
                         float* o = (float*)p.out + at;
 #pragma unroll
@@ -506,11 +508,13 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
     Q6K_REQUIRE(total < (1LL << 31), "gemm_i8: %lld tiles", total);
     t.w_once = p.offsets ? p.rows <= 2LL * p.groups * BT : t.n_y == 1;
     const size_t smem = (size_t)t.stages * stage + extra + 1024;
-    static bool configured = false;
-    if (!configured) {
+    static std::atomic<unsigned long long> configured{0};              // a bit for each device
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return q6k_fail("gemm_i8: device %d", device);
+    if (!(configured.load() >> device & 1)) {
         if (cudaFuncSetAttribute(gemm_i8_tc_kernel<BT, CTAS, DUAL, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess)
             return q6k_check_launch("gemm_i8: shared memory attribute");
-        configured = true;
+        configured.fetch_or(1ull << device);
     }
     const int units = sm_count() / CTAS, cluster = SPLIT ? t.split : CTAS;
     Q6K_REQUIRE(!SPLIT || total * cluster <= 0x7fffffff, "gemm_i8: %lld tiles of %d slices", total, cluster);
@@ -571,14 +575,14 @@ Q6K_API int q6k_gemm_i8_status() {
     return v;
 }
 
-// More than a few rows, or groups.  gathered, gathered_scale (with a_rows): int8 [rows, K] and FP32 [rows] of scratch.  tile: rows of a tile, negative for
-// pairs of CTAs (0: chosen here), with 1000 s added for s slices of K.
-int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, float* gathered_scale, int tile, cudaStream_t st) {
+// More than a few rows, or groups.  gathered (with a_rows): rows * (K + 4) bytes of scratch, for the rows that are picked and their scales.
+int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, cudaStream_t st) {
     TcArgs t{p};
     if (p.rows == 0) return 0;
     Q6K_REQUIRE(p.groups <= MAX_GROUPS && (long long)p.groups * p.N < (1LL << 31) - 256, "gemm_i8: %d groups (at most %d) of %d columns", p.groups, MAX_GROUPS, p.N);
     if (p.a_rows) {
-        Q6K_REQUIRE(gathered && gathered_scale && ((uintptr_t)gathered & 15) == 0, "gemm_i8: no scratch for the rows that are picked");
+        Q6K_REQUIRE(gathered && ((uintptr_t)gathered & 15) == 0, "gemm_i8: no scratch for the rows that are picked");
+        float* gathered_scale = (float*)((char*)gathered + (long long)p.rows * p.K);
         q6k_launch(gather_i8_kernel, (p.rows + 7) / 8, 256, 0, st, p.a, p.lda, p.a_scale, p.a_rows, p.rows, p.K, (int8_t*)gathered, gathered_scale);
         if (int rc = q6k_check_launch("gemm_i8: gather")) return rc;
         t.p.a = (const int8_t*)gathered, t.p.a_scale = gathered_scale, t.p.a_rows = nullptr, t.p.lda = p.K, t.p.early = 1;
@@ -586,12 +590,8 @@ int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, float* g
     }
     Q6K_REQUIRE(a_total >= p.rows, "gemm_i8: %d rows of %d", p.rows, a_total);
     const bool dual = p.w2 != nullptr;
-    t.split = 1;
-    if (tile == 0) tile = choose_tile(t.p, dual, &t.split);
-    else if (tile > 1000) t.split = tile / 1000, tile %= 1000;
+    const int tile = choose_tile(t.p, dual, &t.split);
     if (t.split > 1) {
-        const int kbs = (p.K + BK - 1) / BK;
-        Q6K_REQUIRE(!p.offsets && t.split <= 8 && (t.split - 1) * ((kbs + t.split - 1) / t.split) < kbs, "gemm_i8: K=%d in %d slices", p.K, t.split);
         if (tile == 32) return dual ? launch<32, 1, true, true>(t, a_total, st) : launch<32, 1, false, true>(t, a_total, st);
         if (tile == 64) return dual ? launch<64, 1, true, true>(t, a_total, st) : launch<64, 1, false, true>(t, a_total, st);
         if (tile == 128) return dual ? launch<128, 1, true, true>(t, a_total, st) : launch<128, 1, false, true>(t, a_total, st);

@@ -2045,7 +2045,7 @@ _p, _t = ctypes.c_void_p, ctypes.c_int
 _I8_OPERANDS = [_p, _ll, _p, _t, _p, _p, _p, _p, _t, _t, _p, _p, _t, _p, _t, _p, _ll, _t, _f, _t]
 _ARGTYPES.update({
     "q6k_quantize_rows": [_p, _ll, _t, _t, _t, _p, _p, _p],
-    "q6k_gemm_i8": _I8_OPERANDS + [_t, _p, _p, _t, _p],
+    "q6k_gemm_i8": _I8_OPERANDS + [_t, _p, _p],
     "q6k_linear_i8": [_p, _ll, _t, _t, _p] + _I8_OPERANDS + [_p],
     "q6k_beam_select": [_p, _p, _t, _t, _t, _t, _p, _ll, _p, _p, _p, _p],
     "q6k_reorder_pages": [_t, _p, _p, _p, _p, _p, _t, _t, _t, _t, _p, _p, _p, _p],
@@ -2098,7 +2098,7 @@ def quantize_rows(x: torch.Tensor):
     device = _here(("x", x))
     pitch = _row_pitch(x, "x")
     R, K = x.shape
-    if K < 1 or R > 2 ** 31 - 1 or K > 2 ** 31 - 1:
+    if K < 1 or R >= 1 << 31 or K > 1 << 30:
         raise KernelError(f"quantize_rows: {R} rows of {K} values")
     q = torch.empty((R, K), dtype=torch.int8, device=x.device)
     scale = torch.empty((R,), dtype=torch.float32, device=x.device)
@@ -2141,7 +2141,6 @@ def _data(t: Optional[torch.Tensor]) -> int:
 
 
 _I8_FEW_ROWS = 16                        # products of at most this many rows take the kernel that streams weights past mma.sync
-_i8_tile = 0                             # rows of a tile for measurements (0: the library's rule)
 
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -2173,11 +2172,11 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
         raise KernelError("gemm_i8: the rows of a must start on 16 bytes")
     if grouped:
         _is(offsets, "offsets", torch.int32, (groups + 1,))
-    gathered = gathered_scale = None
-    if a_rows is not None and (grouped or rows > _I8_FEW_ROWS or _i8_tile):
-        gathered, gathered_scale = torch.empty((rows, K), dtype=torch.int8, device=a.device), torch.empty(rows, dtype=torch.float32, device=a.device)
+    gathered = None                      # the rows that are picked, side by side, and their scales
+    if a_rows is not None and (grouped or rows > _I8_FEW_ROWS):
+        gathered = torch.empty(rows * (K + 4), dtype=torch.uint8, device=a.device)
     _call("q6k_gemm_i8", a.data_ptr(), lda, a_scale.data_ptr(), rows, w.data_ptr(), w_scale.data_ptr(), _data(w2), _data(w2_scale), N, K, _data(a_rows), _data(offsets),
-          groups, 0, 1, out.data_ptr(), N, epi, _act_param(act), early, total, _data(gathered), _data(gathered_scale), _i8_tile, _stream_of(device),
+          groups, 0, 1, out.data_ptr(), N, epi, _act_param(act), early, total, _data(gathered), _stream_of(device),
           launches=0 if rows == 0 else 1 if gathered is None else 2)
     return out
 
