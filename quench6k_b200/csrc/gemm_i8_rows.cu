@@ -84,6 +84,22 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
             __syncthreads();
         }
     };
+    // thread -> (column block, row block, element of the fragment, lane of the fragment): columns quad (+8), rows 2 pair (+1).  The scales of a thread's
+    // results are asked for with the first weights and rows, so that they are there when the sums are.
+    constexpr int OUTS = RB * NB * 4 * 32, ITERS = (OUTS + R8_WARPS * 32 - 1) / (R8_WARPS * 32);
+    auto result = [&](int it, int& idx, int& n, int& r) {
+        idx = it * R8_WARPS * 32 + threadIdx.x;
+        const int ln = idx & 31, i = (idx >> 5) & 3, nb = (idx >> 7) % NB, rb = (idx >> 7) / NB;
+        n = n0 + rb * 16 + (ln >> 2) + 8 * (i >> 1), r = nb * 8 + 2 * (ln & 3) + (i & 1);
+        return idx < OUTS && n < p.N && r < rows;
+    };
+    float ws[ITERS], ws2[ITERS], xs[ITERS];
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        int idx, n, r;
+        const bool mine = result(it, idx, n, r);
+        ws[it] = mine ? p.w_scale[first + n] : 0.0f, ws2[it] = DUAL && mine ? p.w2_scale[first + n] : 0.0f;
+    }
     const int8_t* xrow[NB];
     bool live[NB], first_turn = true;
     int acc[MATS][RB][NB][4] = {};
@@ -110,6 +126,11 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
                 live[nb] = nb * 8 + quad < rows;
                 if (HERE) xrow[nb] = row8 + pair * 16;
                 else xrow[nb] = p.a + source(live[nb] ? row0 + nb * 8 + quad : row0) * p.lda + pair * 16;
+            }
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it) {
+                int idx, n, r;
+                xs[it] = HERE ? scale : result(it, idx, n, r) ? p.a_scale[source(row0 + r)] : 0.0f;
             }
         }
 #pragma unroll
@@ -141,20 +162,17 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
 #pragma unroll
                 for (int i = 0; i < 4; ++i) meet[warp][(((m * RB + rb) * NB + nb) * 4 + i) * 32 + lane] = acc[m][rb][nb][i];
     __syncthreads();
-    for (int idx = threadIdx.x; idx < RB * NB * 4 * 32; idx += R8_WARPS * 32) {
-        const int ln = idx & 31, i = (idx >> 5) & 3, nb = (idx >> 7) % NB, rb = (idx >> 7) / NB;
-        const int n = n0 + rb * 16 + (ln >> 2) + 8 * (i >> 1), r = nb * 8 + 2 * (ln & 3) + (i & 1);
-        if (n >= p.N || r >= rows) continue;
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        int idx, n, r;
+        if (!result(it, idx, n, r)) continue;
         int s = 0, s2 = 0;
 #pragma unroll
         for (int q = 0; q < R8_WARPS; ++q) {
             s += meet[q][idx];
-            if (DUAL) s2 += meet[q][RB * NB * 4 * 32 + idx];
+            if (DUAL) s2 += meet[q][OUTS + idx];
         }
-        const float xs = HERE ? scale : p.a_scale[source(row0 + r)];
-        const float v = (float)s * (xs * p.w_scale[first + n]);
-        const float u = DUAL ? (float)s2 * (xs * p.w2_scale[first + n]) : 0.0f;
-        i8_store<DUAL>(p, (long long)(row0 + r) * p.ldo + n, v, u);
+        i8_store<DUAL>(p, (long long)(row0 + r) * p.ldo + n, (float)s * (xs[it] * ws[it]), DUAL ? (float)s2 * (xs[it] * ws2[it]) : 0.0f);
     }
 }
 
@@ -163,23 +181,31 @@ void launch(const I8Args& p, int pairs, cudaStream_t st) {
     q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS, false>, dim3((p.N + RB * 16 - 1) / (RB * 16), pairs), R8_WARPS * 32, 0, st, p);
 }
 
+// Whether rows (not pairs) come here rather than to the tensor-memory kernel: up to eight, or sixteen against a matrix of less than 32 MB (16 rows: 2,048 x
+// 2,048 4.0 us here and 7.0 there, 5,120 x 2,048 7.1 and 9.0; 32,768 x 2,048 20 and 15, 151,936 x 2,048 64 and 52).
+bool few_rows(const I8Args& p) { return p.rows <= 8 || (p.rows <= R8_ROWS && (long long)p.N * p.K * (p.w2 ? 2 : 1) < (32LL << 20)); }
+
+// Columns and loads of a block.  Measured in a graph, weights from HBM (columns x loads a row; the first is taken):
+//   one matrix: 4 loads of 16 columns (8 rows, 32,768 x 2,048: 15.6 us, 2 x 32 columns 17.3; 151,936 x 2,048: 54, 61), 8 where rows are long and blocks few (2,048 x
+//   8,192: 6.6, with four 8.2);
+//   a gated pair of matrices: 2 loads of 32 columns where blocks are many (2 x 8,192 x 2,048: 9.6, 4 of 16 10.2);
+//   pairs, a gated pair of matrices: 2 of 32 (64 pairs, 2 x 512 x 2,048: 23.7, 4 of 16 26.9); one: 1 of 64 where blocks are many (64 pairs, 2,048 x 512: 20.5, 4 of 16 38).
 int launch_rows(const I8Args& p, cudaStream_t st) {
     if (p.rows == 0) return 0;
     Q6K_REQUIRE(!p.offsets && p.rows <= (p.pair_expert ? 65535 : R8_ROWS), "gemm_i8_rows: %d rows", p.rows);
-    const int pairs = p.pair_expert ? p.rows : 1, row_blocks = p.pair_expert || p.rows <= 8 ? 1 : 2;
-    // 32 columns a block where that leaves every SM two of them; long rows of few blocks: eight loads a row at once
-    const bool wide = (long long)p.N * pairs >= 148 * 2 * 32, deep = p.K >= 8192 && !wide;
+    const int pairs = p.pair_expert ? p.rows : 1, two = p.pair_expert || p.rows <= 8 ? 1 : 2;      // blocks of eight rows
+    const long long blocks = (long long)((p.N + 15) / 16) * pairs;                               // of 16 columns
+    const bool deep = p.K >= 8192 && blocks < 4 * 148;
     if (p.w2) {
-        if (row_blocks == 1) launch<true, 1, 1, 4>(p, pairs, st);
-        else launch<true, 2, 1, 4>(p, pairs, st);
-    } else if (row_blocks == 1) {
-        if (wide) launch<false, 1, 2, 4>(p, pairs, st);
-        else if (deep) launch<false, 1, 1, 8>(p, pairs, st);
-        else launch<false, 1, 1, 4>(p, pairs, st);
-    } else {
+        if (two == 2) launch<true, 2, 1, 4>(p, pairs, st);
+        else if (p.pair_expert || blocks >= 4 * 148) launch<true, 1, 2, 2>(p, pairs, st);
+        else launch<true, 1, 1, 4>(p, pairs, st);
+    } else if (p.pair_expert && p.K <= 2048 && blocks >= 8 * 148) launch<false, 1, 4, 1>(p, pairs, st);
+    else if (two == 2) {
         if (deep) launch<false, 2, 1, 8>(p, pairs, st);
         else launch<false, 2, 1, 4>(p, pairs, st);
-    }
+    } else if (deep) launch<false, 1, 1, 8>(p, pairs, st);
+    else launch<false, 1, 1, 4>(p, pairs, st);
     return q6k_check_launch("gemm_i8_rows");
 }
 
@@ -188,13 +214,13 @@ int launch_rows(const I8Args& p, cudaStream_t st) {
 int q6k_quantize_rows_launch(const void* x, long long ldx, int R, int K, int dtype, void* q, float* scale, cudaStream_t st);
 int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, cudaStream_t st);
 
-// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered: rows * (K + 4) bytes of scratch, where a_rows comes with more than 16 rows or with
+// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered: rows * (K + 4) bytes of scratch, where a_rows comes with more than eight rows or with
 // groups.
 Q6K_API int q6k_gemm_i8(I8_OPERANDS, int a_total, void* gathered, cudaStream_t st) {
     I8Args p;
     if (int rc = i8_args(&p, "gemm_i8", I8_NAMES)) return rc;
     Q6K_REQUIRE(!pair_expert, "gemm_i8: pairs come with rows that are not in 8 bits");
-    if (rows <= R8_ROWS && !offsets) return launch_rows(p, st);
+    if (!offsets && few_rows(p)) return launch_rows(p, st);
     return q6k_gemm_i8_tc_launch(p, a_total, gathered, st);
 }
 
@@ -213,7 +239,7 @@ Q6K_API int q6k_linear_i8(const void* x, long long ldx, int T, int dtype, void* 
         return rc;
     Q6K_REQUIRE(!offsets && !a_rows && (pair_expert ? (rows + pair_div - 1) / pair_div <= T : rows == T), "linear_i8: %d rows of %d", rows, T);
     if (rows == 0) return 0;
-    const bool few = pair_expert || rows <= R8_ROWS;
+    const bool few = pair_expert || few_rows(p);
     if (q6k_linear_i8_scratch(T, N, K, dtype, ((uintptr_t)x & 15) == 0, pair_expert != nullptr) == 0) {
         p.x = (const __nv_bfloat16*)x, p.early = early;
         const int blocks = (N + 15) / 16;

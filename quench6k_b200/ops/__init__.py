@@ -2140,7 +2140,6 @@ def _data(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-_I8_FEW_ROWS = 16                        # products of at most this many rows take the kernel that streams weights past mma.sync
 
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -2173,7 +2172,7 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     if grouped:
         _is(offsets, "offsets", torch.int32, (groups + 1,))
     gathered = None                      # the rows that are picked, side by side, and their scales
-    if a_rows is not None and (grouped or rows > _I8_FEW_ROWS):
+    if a_rows is not None and (grouped or rows > 8):
         gathered = torch.empty(rows * (K + 4), dtype=torch.uint8, device=a.device)
     _call("q6k_gemm_i8", a.data_ptr(), lda, a_scale.data_ptr(), rows, w.data_ptr(), w_scale.data_ptr(), _data(w2), _data(w2_scale), N, K, _data(a_rows), _data(offsets),
           groups, 0, 1, out.data_ptr(), N, epi, _act_param(act), early, total, _data(gathered), _stream_of(device),

@@ -115,7 +115,7 @@ GATED = BF16_HALF + (3 * 201 + 3 + 10 + 201) * HALF
 
 SHAPES = [(1, 1, 16), (1, 2048, 2048), (2, 100, 48), (3, 17, 1024), (8, 64, 64), (9, 4097, 80), (16, 129, 4096), (17, 128, 128), (32, 1000, 2048), (33, 257, 272),
           (64, 384, 512), (100, 640, 1040), (129, 300, 144), (200, 129, 8192), (257, 512, 2064), (300, 7, 16), (1000, 1024, 256),
-          (17, 512, 10240), (100, 200, 8208), (48, 2048, 8192), (250, 1100, 4112), (130, 90, 1168)]      # few tiles and long rows: K in slices
+          (17, 512, 10240), (100, 200, 8208), (48, 2048, 8192), (250, 1100, 4112), (130, 90, 1168), (13, 17000, 2048), (8, 17000, 2048)]      # few tiles and long rows: K in slices
 
 
 @pytest.mark.parametrize("rows,n,k", SHAPES)
@@ -192,7 +192,7 @@ def test_grouped_product(counts, n, k, gated):
 
 
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("tokens,top,n,k", [(1, 8, 512, 2048), (3, 2, 33, 80), (16, 4, 128, 1024), (5, 1, 7, 16)])
+@pytest.mark.parametrize("tokens,top,n,k", [(1, 8, 512, 2048), (3, 2, 33, 80), (16, 4, 128, 1024), (5, 1, 7, 16), (16, 8, 200, 512), (16, 8, 170, 2064)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_product_pair_by_pair(tokens, top, n, k, gated, dtype):
     """One row for each (token, expert); a pair that names no matrix is left as it was."""
@@ -272,6 +272,15 @@ def test_a_row_that_is_not_finite_makes_its_results_nan_and_no_other(rows):
     _, _, ((w, t),) = operands(6, 1, 200, 256)
     y = ops.linear_i8(x, w.cuda(), t.cuda())
     assert bool(y[1].isnan().all()) and not bool(y[[i for i in range(rows) if i != 1]].isnan().any())
+
+
+@pytest.mark.parametrize("rows,n", [(5, 100), (12, 100), (12, 33000), (40, 100)])
+def test_rows_that_are_picked(rows, n):
+    """Without groups: some twice, some not at all."""
+    from quench6k_b200 import ops
+    a, s, ((w, t),) = operands(rows, 20, n, 1024)
+    pick = torch.randint(0, 20, (rows,), generator=torch.Generator().manual_seed(rows), dtype=torch.int32)
+    near(ops.gemm_i8(a.cuda(), s.cuda(), w.cuda(), t.cuda(), a_rows=pick.cuda()), product64(a[pick.long()], s[pick.long()], w, t), STORED)
 
 
 @pytest.mark.parametrize("rows", [4, 200])
