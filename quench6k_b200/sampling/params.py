@@ -2,6 +2,7 @@
 (crates/engine/src/session.rs:14-41; DOCS.md "Request fields")."""
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import List, Optional
 
@@ -61,6 +62,8 @@ class BeamParams:
             raise ValueError("width must be in 1..32")
         if self.max_tokens < 1:
             raise ValueError("max_tokens must be at least 1")
+        if not math.isfinite(self.length_penalty) or abs(self.length_penalty) * math.log(self.max_tokens) > 700.0:
+            raise ValueError("length_penalty must be finite, and a length to its power a number")
         if self.num_return is not None and not 1 <= self.num_return <= self.width:
             raise ValueError("num_return must be in 1..width")
         if self.width * (1 + len(set(self.stop_tokens))) > 128:

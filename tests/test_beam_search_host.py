@@ -115,6 +115,13 @@ class _Runner:
         self.vocab_size = 50
 
 
+def test_powers_of_a_length_that_are_no_numbers_are_refused():
+    for bad in (float("inf"), float("nan"), 400.0, -400.0):
+        with pytest.raises(ValueError, match="length_penalty"):
+            BeamParams(length_penalty=bad, max_tokens=64).validate()
+    BeamParams(length_penalty=400.0, max_tokens=1).validate()
+
+
 def test_prompts_run_as_many_at_a_time_as_fit():
     # two beams of 6 + 4 tokens: 3 pages each
     params = BeamParams(width=2, max_tokens=4)
