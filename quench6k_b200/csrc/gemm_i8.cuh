@@ -17,6 +17,7 @@ struct I8Args {
     int epilogue, act;
     float act_param;
     const __nv_bfloat16* x;        // not null: the one row of a and its scale are still to be made from this
+    int a_total;                   // with a_rows: the rows of a; a number outside them gives a row of NaN
 };
 
 namespace {
@@ -34,7 +35,7 @@ inline int i8_args(I8Args* p, const char* who, I8_OPERANDS) {
     Q6K_REQUIRE(act >= 0 && act <= (epi == I8_GATED ? Q6K_ACT_CLAMPED : 2), "%s: unknown activation %d", who, act);
     Q6K_REQUIRE(!(offsets && pair_expert) && groups >= 1 && pair_div >= 1, "%s: groups %d, pair_div %d", who, groups, pair_div);
     *p = I8Args{(const int8_t*)a, (const int8_t*)w, (const int8_t*)w2, a_scale, w_scale, w2_scale, a_rows, offsets, pair_expert, out, lda, ldo,
-                rows, N, K, groups, pair_div, early, epi, act, act_param, nullptr};
+                rows, N, K, groups, pair_div, early, epi, act, act_param, nullptr, 0};
     return 0;
 }
 

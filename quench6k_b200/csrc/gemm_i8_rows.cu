@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
             if (DUAL) wrow[1][rb][h] = p.w2 + r * p.K + pair * 16;
         }
     auto source = [&](int r) -> long long { return p.pair_expert ? r / p.pair_div : p.a_rows ? p.a_rows[r] : r; };
+    auto is_row = [&](long long r) { return !p.a_rows || (unsigned long long)r < (unsigned long long)p.a_total; };
     // every thread of the block once: the row in 8 bits to shared memory
     auto take_row = [&] {
         if constexpr (HERE) {
@@ -125,12 +126,20 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
             for (int nb = 0; nb < NB; ++nb) {
                 live[nb] = nb * 8 + quad < rows;
                 if (HERE) xrow[nb] = row8 + pair * 16;
-                else xrow[nb] = p.a + source(live[nb] ? row0 + nb * 8 + quad : row0) * p.lda + pair * 16;
+                else {
+                    const long long from = source(live[nb] ? row0 + nb * 8 + quad : row0);
+                    live[nb] = live[nb] && is_row(from);
+                    xrow[nb] = p.a + (live[nb] ? from : 0) * p.lda + pair * 16;
+                }
             }
 #pragma unroll
             for (int it = 0; it < ITERS; ++it) {
                 int idx, n, r;
-                xs[it] = HERE ? scale : result(it, idx, n, r) ? p.a_scale[source(row0 + r)] : 0.0f;
+                if (HERE) xs[it] = scale;
+                else if (result(it, idx, n, r)) {
+                    const long long from = source(row0 + r);
+                    xs[it] = is_row(from) ? p.a_scale[from] : __uint_as_float(0x7fffffffu);
+                } else xs[it] = 0.0f;
             }
         }
 #pragma unroll
@@ -220,6 +229,7 @@ Q6K_API int q6k_gemm_i8(I8_OPERANDS, int a_total, void* gathered, cudaStream_t s
     I8Args p;
     if (int rc = i8_args(&p, "gemm_i8", I8_NAMES)) return rc;
     Q6K_REQUIRE(!pair_expert, "gemm_i8: pairs come with rows that are not in 8 bits");
+    p.a_total = a_total;
     if (!offsets && few_rows(p)) return launch_rows(p, st);
     return q6k_gemm_i8_tc_launch(p, a_total, gathered, st);
 }

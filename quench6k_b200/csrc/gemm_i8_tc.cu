@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
             const int span = tl.n == BT ? SPAN : (tl.n / (EW / 4) + 31) / 32 * 32, row0 = tl.row0 + part * span;      // this warp's rows of the tile
             const int end = min(span, tl.row_end - row0);
             // the rows' scales go to shared memory while the accumulator fills (read from global memory where they are needed, every 16 rows waited for them:
-            // 2,048 x 2,048 x 2,048 16.0 us, 12.1 now)
+            // 2,048 x 2,048 x 2,048 16.0 us, 15.4 that way)
             const uint32_t scales = scales0 + (warp - 2) * SCALE_BYTES;
             __syncwarp();
 #pragma unroll
@@ -443,20 +443,21 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     }
 }
 
-// Rows picked from a with their scales, a warp each, so that the tiles' loads find them side by side.
-__global__ void __launch_bounds__(256) gather_i8_kernel(const int8_t* a, long long lda, const float* a_scale, const int* a_rows, int rows, int K, int8_t* out, float* scale) {
+// Rows picked from a with their scales, a warp each, so that the tiles' loads find them side by side (a number outside a: zeros and the scale NaN).
+__global__ void __launch_bounds__(256) gather_i8_kernel(const int8_t* a, long long lda, const float* a_scale, const int* a_rows, int a_total, int rows, int K, int8_t* out, float* scale) {
     pdl_enter();
     const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (r >= rows) return;
     const int from = a_rows[r];
+    const bool is_row = (unsigned)from < (unsigned)a_total;
     const int8_t* src = a + from * lda;
     int8_t* dst = out + (long long)r * K;
-    if (lane == 0) scale[r] = a_scale[from];
+    if (lane == 0) scale[r] = is_row ? a_scale[from] : __uint_as_float(0x7fffffffu);
     for (int k0 = lane * 16; k0 < K; k0 += 4 * 512) {
         uint4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (k0 + i * 512 < K) v[i] = *(const uint4*)(src + k0 + i * 512);
+            if (k0 + i * 512 < K) v[i] = is_row ? *(const uint4*)(src + k0 + i * 512) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (k0 + i * 512 < K) *(uint4*)(dst + k0 + i * 512) = v[i];
@@ -583,7 +584,7 @@ int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, cudaStre
     if (p.a_rows) {
         Q6K_REQUIRE(gathered && ((uintptr_t)gathered & 15) == 0, "gemm_i8: no scratch for the rows that are picked");
         float* gathered_scale = (float*)((char*)gathered + (long long)p.rows * p.K);
-        q6k_launch(gather_i8_kernel, (p.rows + 7) / 8, 256, 0, st, p.a, p.lda, p.a_scale, p.a_rows, p.rows, p.K, (int8_t*)gathered, gathered_scale);
+        q6k_launch(gather_i8_kernel, (p.rows + 7) / 8, 256, 0, st, p.a, p.lda, p.a_scale, p.a_rows, a_total, p.rows, p.K, (int8_t*)gathered, gathered_scale);
         if (int rc = q6k_check_launch("gemm_i8: gather")) return rc;
         t.p.a = (const int8_t*)gathered, t.p.a_scale = gathered_scale, t.p.a_rows = nullptr, t.p.lda = p.K, t.p.early = 1;
         a_total = p.rows;

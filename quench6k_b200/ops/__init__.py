@@ -2140,8 +2140,6 @@ def _data(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-
-
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
             accumulate: bool = False, w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None,
             offsets: Optional[torch.Tensor] = None, a_rows: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
@@ -2150,7 +2148,7 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     a: int8 [*, K] (its rows may lie apart), a_scale: float32 [*]; w: int8 [N, K] with w_scale float32 [N]; K a multiple of 16 below
     131,072.  Stored in float32, or added into `out` (accumulate).  With w2 the gated epilogue act(y) * y2 (act None: silu), with
     act alone act(y); both leave in bfloat16.
-    a_rows (int32 [rows]): row r of the product is row a_rows[r] of a.  offsets (int32 [G + 1], ascending from 0) with w [G, N, K]
+    a_rows (int32 [rows]): row r of the product is row a_rows[r] of a (a number outside a: a row of NaN).  offsets (int32 [G + 1], ascending from 0) with w [G, N, K]
     and w_scale [G, N]: rows offsets[g] .. offsets[g + 1] - 1 go against matrix g; rows behind the last offset are left as they were.
     early: the caller's word that the kernel before this call made a and a_scale and nothing else that is read here: the weights
     are then fetched while it ends."""

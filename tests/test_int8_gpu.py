@@ -283,6 +283,19 @@ def test_rows_that_are_picked(rows, n):
     near(ops.gemm_i8(a.cuda(), s.cuda(), w.cuda(), t.cuda(), a_rows=pick.cuda()), product64(a[pick.long()], s[pick.long()], w, t), STORED)
 
 
+@pytest.mark.parametrize("rows,n", [(5, 100), (12, 33000), (40, 100)])
+def test_a_picked_row_that_is_none_is_a_row_of_nan(rows, n):
+    from quench6k_b200 import ops
+    a, s, ((w, t),) = operands(rows, 20, n, 256)
+    pick = torch.randint(0, 20, (rows,), generator=torch.Generator().manual_seed(rows), dtype=torch.int32)
+    bad = torch.zeros(rows, dtype=torch.bool)
+    pick[0], pick[2], pick[4] = -1, 20, 2 ** 31 - 1
+    bad[[0, 2, 4]] = True
+    y = ops.gemm_i8(a.cuda(), s.cuda(), w.cuda(), t.cuda(), a_rows=pick.cuda()).cpu()
+    assert bool(y[bad].isnan().all())
+    near(y[~bad], product64(a[pick[~bad].long()], s[pick[~bad].long()], w, t), STORED)
+
+
 @pytest.mark.parametrize("rows", [4, 200])
 def test_operands_whose_rows_lie_apart(rows):
     from quench6k_b200 import ops
