@@ -113,12 +113,12 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
 #pragma unroll
             for (int j = 0; j < SEL_EACH; j += 4) {
                 const int i = where(threadIdx.x, j);
-                const float4 f = i < n ? __ldg((const float4*)(tile + i)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                const float4 f = i < n ? *(const float4*)(tile + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                 v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < SEL_EACH; ++j) v[j] = where(threadIdx.x, j) < n ? __ldg(tile + where(threadIdx.x, j)) : -INFINITY;
+            for (int j = 0; j < SEL_EACH; ++j) v[j] = where(threadIdx.x, j) < n ? tile[where(threadIdx.x, j)] : -INFINITY;
         }
         float high = -INFINITY;
 #pragma unroll
