@@ -38,6 +38,7 @@ struct TcArgs {
     int stages, n_x, n_y;              // tiles along N, and along the rows (dense)
     int w_once;                        // every weight tile is fetched once, or by few units side by side
     int split;                         // SPLIT: CTAs of a cluster, which share a tile's K
+    int whole, cut;                    // dense: tiles that are taken whole, and into how many pieces along the rows each of the others is cut
 };
 
 // D: 32-bit integers, A and B signed 8-bit integers, both K-major, M rows, N = n.
@@ -102,6 +103,11 @@ struct Tile {
 template <int BT, int CTAS>
 __device__ __forceinline__ Tile tile_of(const TcArgs& a, int t, int cols, const int* starts) {
     Tile o;
+    int rows = BT, skip = 0;                             // of the tile: which rows of it are meant
+    if (!a.p.offsets && t >= a.whole) {                  // the last round of a dense product
+        const int u = t - a.whole;
+        rows = BT / a.cut, skip = u % a.cut * rows, t = a.whole + u / a.cut;
+    }
     const int y = t / a.n_x;
     o.n0 = t % a.n_x * cols;
     if (a.p.offsets) {
@@ -115,9 +121,9 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, int t, int cols, const 
         const int* offsets = starts + a.p.groups + 1;
         o.row0 = offsets[lo] + (y - starts[lo]) * BT, o.row_end = offsets[lo + 1];
     } else {
-        o.g = 0, o.row0 = y * BT, o.row_end = a.p.rows;
+        o.g = 0, o.row0 = y * BT + skip, o.row_end = min(a.p.rows, o.row0 + rows);
     }
-    o.n = min(BT, (o.row_end - o.row0 + 32 * CTAS - 1) / (32 * CTAS) * (32 * CTAS));
+    o.n = max(32 * CTAS, min(BT, (o.row_end - o.row0 + 32 * CTAS - 1) / (32 * CTAS) * (32 * CTAS)));      // (a piece behind the last row is multiplied with zeros)
     return o;
 }
 
@@ -189,7 +195,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(BT), 1) gemm_i8_tc_ke
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     pdl_launch();                                        // this block holds its tensor memory: a successor may come
-    const int total = a.n_x * (p.offsets ? starts[p.groups] : a.n_y), kb_all = (p.K + BK - 1) / BK;
+    const int total = p.offsets ? a.n_x * starts[p.groups] : a.whole + (a.n_x * a.n_y - a.whole) * a.cut, kb_all = (p.K + BK - 1) / BK;
     // the k-blocks of this CTA: kb0 .. kb0 + kbs - 1 (SPLIT: one tile for each cluster, and every slice has some)
     const int slice = SPLIT ? (int)cluster_rank() : 0, slice_kbs = SPLIT ? (kb_all + a.split - 1) / a.split : kb_all;
     const int kb0 = slice * slice_kbs, kbs = min(slice_kbs, kb_all - kb0);
@@ -506,7 +512,9 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
     if (t.stages > MAX_STAGES) t.stages = MAX_STAGES;
     t.n_x = (p.N + COLS - 1) / COLS, t.n_y = (p.rows + BT - 1) / BT;
     const long long row_tiles = p.offsets ? p.rows / BT + (p.groups < p.rows ? p.groups : p.rows) : t.n_y, total = t.n_x * row_tiles;
-    Q6K_REQUIRE(total < (1LL << 31), "gemm_i8: %lld tiles", total);
+    const int units = sm_count() / CTAS;
+    Q6K_REQUIRE(total < (1LL << 31) - 2 * 148, "gemm_i8: %lld tiles", total);
+    t.whole = t.cut > 1 ? (int)(total - total % units) : (int)total;
     t.w_once = p.offsets ? p.rows <= 2LL * p.groups * BT : t.n_y == 1;
     const size_t smem = (size_t)t.stages * stage + extra + 1024;
     static std::atomic<unsigned long long> configured{0};              // a bit for each device
@@ -517,10 +525,11 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
             return q6k_check_launch("gemm_i8: shared memory attribute");
         configured.fetch_or(1ull << device);
     }
-    const int units = sm_count() / CTAS, cluster = SPLIT ? t.split : CTAS;
+    const int cluster = SPLIT ? t.split : CTAS;
     Q6K_REQUIRE(!SPLIT || total * cluster <= 0x7fffffff, "gemm_i8: %lld tiles of %d slices", total, cluster);
+    const long long pieces = p.offsets ? total : t.whole + (total - t.whole) * t.cut;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster * (unsigned)(SPLIT || total < units ? total : units)), cfg.blockDim = dim3(64 + 32 * EW), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.gridDim = dim3(cluster * (unsigned)(SPLIT || pieces < units ? pieces : units)), cfg.blockDim = dim3(64 + 32 * EW), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr[2];
     if (cluster > 1) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
@@ -544,8 +553,11 @@ int launch(const TcArgs& args, int a_total, cudaStream_t st) {
 // Grouped rows: the experts' shares are known on the device only, so half as much again as an even share.
 // split: CTAs that share a tile's K, where that takes less time: a slice's share of it and two microseconds for the sums to meet (2,048 columns, K 8,192,
 // 32 rows: 16.8 us in 16 CTAs, 10.3 in four slices; K 2,048: 7.0 and 7.0, in two 8.4).
-int choose_tile(const I8Args& p, bool dual, int* split) {
-    *split = 1;
+// cut: the pieces along the rows of each tile of the last round, where its tiles fill less than half of the units (1,522 rows x (2 x 8,192): 14 tiles over 74
+// pairs as 56 pieces of 64 rows, 42.0 -> 40.6 us; 2,048 rows x 8,192 33.8 -> 32.3).  A piece takes longer than a narrow tile of a product of narrow tiles: with their
+// times 1,300 x 4,096, K 4,096 was cut, too, and took 25.5 us instead of 23.6.
+int choose_tile(const I8Args& p, bool dual, int* split, int* cut) {
+    *split = *cut = 1;
     if (p.offsets) {
         const int share = p.rows / p.groups + p.rows / p.groups / 2;
         return share <= 32 ? 32 : share <= 64 ? 64 : 128;
@@ -558,11 +570,17 @@ int choose_tile(const I8Args& p, bool dual, int* split) {
         const long long units = sm_count() / ctas, count = (long long)((p.N + cols - 1) / cols) * ((p.rows + bt - 1) / bt);
         const int kbs = (p.K + BK - 1) / BK;
         const long long cost = (count + units - 1) / units * t[1] * kbs;                  // in units of a sixteenth of a tenth of a microsecond
-        if (best < 0 || cost < best) best = cost, pick = t[0], *split = 1;
+        if (best < 0 || cost < best) best = cost, pick = t[0], *split = *cut = 1;
+        for (int c = 2; count > units && bt / c >= 32 * ctas && count % units * c <= units; ++c) {
+            if (count % units == 0 || bt % c || bt / c % (32 * ctas)) continue;
+            const int piece = bt / c / ctas;                                             // rows that each CTA loads for one
+            const long long with = (count / units * t[1] + (piece <= 32 ? 48 : piece <= 64 ? 52 : 56)) * kbs;
+            if (with < best) best = with, pick = t[0], *split = 1, *cut = c;
+        }
         // clusters whose CTAs all run at a time: 96 in eights, 128 in fours and twos (of 148 SMs; 16 clusters of eight took two rounds)
         for (int s = 2; ctas == 1 && bt <= 128 && s <= 8 && count * s <= (s == 8 ? 96 : 128) && (s - 1) * ((kbs + s - 1) / s) < kbs; s *= 2) {
-            const long long cut = (long long)t[1] * ((kbs + s - 1) / s) + 16 * 20;
-            if (cut < best) best = cut, pick = t[0], *split = s;
+            const long long sliced = (long long)t[1] * ((kbs + s - 1) / s) + 16 * 20;
+            if (sliced < best) best = sliced, pick = t[0], *split = s, *cut = 1;
         }
     }
     return pick;
@@ -591,7 +609,7 @@ int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, cudaStre
     }
     Q6K_REQUIRE(a_total >= p.rows, "gemm_i8: %d rows of %d", p.rows, a_total);
     const bool dual = p.w2 != nullptr;
-    const int tile = choose_tile(t.p, dual, &t.split);
+    const int tile = choose_tile(t.p, dual, &t.split, &t.cut);
     if (t.split > 1) {
         if (tile == 32) return dual ? launch<32, 1, true, true>(t, a_total, st) : launch<32, 1, false, true>(t, a_total, st);
         if (tile == 64) return dual ? launch<64, 1, true, true>(t, a_total, st) : launch<64, 1, false, true>(t, a_total, st);

@@ -153,6 +153,27 @@ def test_gated_product(rows, n, k, act):
     near(y, gated64(g, u, act), GATED, abs_=float(8 * HALF * (g.abs() * (u.abs() + 1)).max()))
 
 
+@pytest.mark.parametrize("rows,n,k,gated", [(129, 20000, 48, False), (193, 20000, 16, False), (961, 11000, 32, False), (2048, 8192, 144, False),
+                                            (129, 11000, 48, True), (385, 11000, 48, True), (1290, 8192, 64, True), (1281, 8192, 128, True)])
+def test_product_whose_last_tiles_are_cut(rows, n, k, gated):
+    """More tiles than run at a time and few in the last round; some pieces of those have no row.  The memory behind the result stays as it was."""
+    from quench6k_b200 import ops
+    a, s, mats = operands(rows + k, rows, n, k, mats=2 if gated else 1)
+    s = s * 0.02
+    (w, t), more = mats[0], {}
+    if gated:
+        more = {"w2": mats[1][0].cuda(), "w2_scale": mats[1][1].cuda()}
+    out = torch.full((rows + 300, n), 7.0, dtype=torch.bfloat16 if gated else torch.float32, device="cuda")
+    ops.gemm_i8(a.cuda(), s.cuda(), w.cuda(), t.cuda(), out=out, **more)
+    g = product64(a, s, w, t)
+    if gated:
+        u = product64(a, s, *mats[1])
+        near(out[:rows], gated64(g, u, None), GATED, 1e-30)
+    else:
+        near(out[:rows], g, STORED)
+    assert bool((out[rows:] == 7.0).all())
+
+
 @pytest.mark.parametrize("act", ["silu", "relu2"])
 @pytest.mark.parametrize("rows,n,k", [(5, 64, 128), (150, 300, 256), (20, 100, 6144)])
 def test_activated_product(rows, n, k, act):
