@@ -185,6 +185,64 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
     }
 }
 
+// Pairs against short rows: a warp takes 16 columns over all of K, so that nothing waits for another warp.  grid (blocks of 16 PAIR_WARPS columns, pairs).
+constexpr int PAIR_WARPS = 4;
+template <bool DUAL, int LOADS>
+__global__ void __launch_bounds__(PAIR_WARPS * 32) gemm_i8_pairs_kernel(const I8Args p) {
+    pdl_launch();
+    constexpr int MATS = DUAL ? 2 : 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, pair = lane & 3;
+    const int n0 = (blockIdx.x * PAIR_WARPS + warp) * 16, row = blockIdx.y;
+    if (!p.early) pdl_wait();
+    const int g = p.pair_expert[row];
+    if ((unsigned)g >= (unsigned)p.groups || n0 >= p.N) {
+        if (p.early) pdl_wait();                          // a warp that ends has waited too: who waits for this kernel counts on it
+        return;
+    }
+    const uint64_t once = l2_evict_first_policy();
+    const long long first = (long long)g * p.N;
+    const int8_t* wrow[MATS][2];
+    float ws[MATS][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const long long r = first + min(n0 + quad + 8 * h, p.N - 1);      // a ragged last block reads a valid row and drops the sums
+        wrow[0][h] = p.w + r * p.K + pair * 16, ws[0][h] = p.w_scale[r];
+        if (DUAL) wrow[MATS - 1][h] = p.w2 + r * p.K + pair * 16, ws[MATS - 1][h] = p.w2_scale[r];
+    }
+    const long long from = row / p.pair_div;
+    const int8_t* xrow = p.a + from * p.lda + pair * 16;
+    float xs = 0.0f;
+    int acc[MATS][4] = {};
+    for (int k0 = 0; k0 < p.K; k0 += 64 * LOADS) {
+        uint4 w[MATS][2][LOADS], x[LOADS];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+#pragma unroll
+            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) w[m][h][j] = k0 + j * 64 + pair * 16 < p.K ? ld_once(wrow[m][h] + k0 + j * 64, once) : make_uint4(0, 0, 0, 0);
+        if (k0 == 0) {
+            if (p.early) pdl_wait();
+            xs = p.a_scale[from];
+        }
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) x[j] = quad == 0 && k0 + j * 64 + pair * 16 < p.K ? ld_after_wait(xrow + k0 + j * 64) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                r8_mma(acc[m], w[m][0][j].x, w[m][1][j].x, w[m][0][j].y, w[m][1][j].y, x[j].x, x[j].y);
+                r8_mma(acc[m], w[m][0][j].z, w[m][1][j].z, w[m][0][j].w, w[m][1][j].w, x[j].z, x[j].w);
+            }
+    }
+    if (pair == 0) {                                      // the lanes with the one row's sums
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (n0 + quad + 8 * h < p.N)
+                i8_store<DUAL>(p, (long long)row * p.ldo + n0 + quad + 8 * h, (float)acc[0][2 * h] * (xs * ws[0][h]), (float)acc[MATS - 1][2 * h] * (xs * ws[MATS - 1][h]));
+    }
+}
+
 template <bool DUAL, int NB, int RB, int LOADS>
 void launch(const I8Args& p, int pairs, cudaStream_t st) {
     q6k_launch_as(p.early != 0, gemm_i8_rows_kernel<DUAL, NB, RB, LOADS, false>, dim3((p.N + RB * 16 - 1) / (RB * 16), pairs), R8_WARPS * 32, 0, st, p);
@@ -197,20 +255,28 @@ bool few_rows(const I8Args& p) { return p.rows <= 8 || (p.rows <= R8_ROWS && (lo
 // Columns and loads of a block.  Measured in a graph, weights from HBM (columns x loads a row; the first is taken):
 //   one matrix: 4 loads of 16 columns (8 rows, 32,768 x 2,048: 15.6 us, 2 x 32 columns 17.3; 151,936 x 2,048: 54, 61), 8 where rows are long and blocks few (2,048 x
 //   8,192: 6.6, with four 8.2);
-//   a gated pair of matrices: 2 loads of 32 columns where blocks are many (2 x 8,192 x 2,048: 9.6, 4 of 16 10.2);
-//   pairs, a gated pair of matrices: 2 of 32 (64 pairs, 2 x 512 x 2,048: 23.7, 4 of 16 26.9); one: 1 of 64 where blocks are many (64 pairs, 2,048 x 512: 20.5, 4 of 16 38).
+//   a gated pair of matrices: 2 loads of 32 columns where blocks are many (2 x 8,192 x 2,048: 9.6, 4 of 16 10.2).
+// Pairs (with the rows' way to 8 bits), warps for themselves or blocks that split K:
+//   one matrix: warps (64 pairs, 2,048 x 512: 14.5 us and 21.4; four pairs 4.3 and 5.7; 16 pairs, 5,120 x 2,048 31.2 and 33.2), 4 loads where K ends there (256 pairs,
+//   2,048 x 256: 22.8, with eight 31.5);
+//   a gated pair: warps where rows are short or warps many (64 pairs, 2 x 1,024 x 512: 14.1 and 20.7; 2 x 512 x 2,048: 23.5 and 24.8), blocks otherwise (8 pairs, 2 x 512 x
+//   2,048: 7.7, warps 11.8; 16 pairs, 2 x 2,048 x 5,120: 54.5, 55.9).
 int launch_rows(const I8Args& p, cudaStream_t st) {
     if (p.rows == 0) return 0;
     Q6K_REQUIRE(!p.offsets && p.rows <= (p.pair_expert ? 65535 : R8_ROWS), "gemm_i8_rows: %d rows", p.rows);
     const int pairs = p.pair_expert ? p.rows : 1, two = p.pair_expert || p.rows <= 8 ? 1 : 2;      // blocks of eight rows
     const long long blocks = (long long)((p.N + 15) / 16) * pairs;                               // of 16 columns
     const bool deep = p.K >= 8192 && blocks < 4 * 148;
-    if (p.w2) {
+    if (p.pair_expert && (!p.w2 || p.K <= 256 || (p.K <= 2048 && blocks >= (p.K <= 1024 ? 5 : 8) * 148))) {
+        const dim3 grid((p.N + PAIR_WARPS * 16 - 1) / (PAIR_WARPS * 16), pairs);
+        if (p.w2) q6k_launch_as(p.early != 0, gemm_i8_pairs_kernel<true, 4>, grid, PAIR_WARPS * 32, 0, st, p);
+        else if (p.K <= 256) q6k_launch_as(p.early != 0, gemm_i8_pairs_kernel<false, 4>, grid, PAIR_WARPS * 32, 0, st, p);
+        else q6k_launch_as(p.early != 0, gemm_i8_pairs_kernel<false, 8>, grid, PAIR_WARPS * 32, 0, st, p);
+    } else if (p.w2) {
         if (two == 2) launch<true, 2, 1, 4>(p, pairs, st);
         else if (p.pair_expert || blocks >= 4 * 148) launch<true, 1, 2, 2>(p, pairs, st);
         else launch<true, 1, 1, 4>(p, pairs, st);
-    } else if (p.pair_expert && p.K <= 2048 && blocks >= 8 * 148) launch<false, 1, 4, 1>(p, pairs, st);
-    else if (two == 2) {
+    } else if (two == 2) {
         if (deep) launch<false, 2, 1, 8>(p, pairs, st);
         else launch<false, 2, 1, 4>(p, pairs, st);
     } else if (deep) launch<false, 1, 1, 8>(p, pairs, st);
