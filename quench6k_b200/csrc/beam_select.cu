@@ -16,7 +16,7 @@ namespace {
 constexpr int SEL_THREADS = 256, SEL_MAX_COUNT = 128, SEL_MAX_WIDTH = 32;
 constexpr int SEL_EACH = 32, SEL_TILE = SEL_THREADS * SEL_EACH;
 constexpr int MERGE_THREADS = 512, MERGE_WARPS = MERGE_THREADS / 32, MERGE_HELD = 4;
-constexpr int SEL_WARPS = SEL_THREADS / 32, SEL_POOL = 1024, SEL_TILES = 8;       // keys that a pool holds; the most tiles of a part
+constexpr int SEL_WARPS = SEL_THREADS / 32, SEL_POOL = 1024, SEL_TILES = 8, SEL_AGAIN = 4;       // keys that a pool holds; the most tiles of a part; pieces that a warp reads again at once
 constexpr int SEL_PARTS = 4;       // parts to an SM that a long batch is cut into (8: 29 us where 4 take 25, 128 rows of 151,936 logits: more parts leave more to merge)
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -164,15 +164,27 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
     for (int t = 0; t < tiles && lo + t * SEL_TILE < hi; ++t)
         if (piece_most[t][threadIdx.x] >= reach && most < INFINITY) pieces[atomicAdd(&listed, 1)] = (unsigned short)(t * SEL_THREADS + threadIdx.x);
     __syncthreads();
-    for (int i = warp; i < listed; i += SEL_WARPS) {
-        const int t = pieces[i] / SEL_THREADS, p = lo + t * SEL_TILE + where(pieces[i] % SEL_THREADS, lane);
-        const float v = p < hi ? row[p] : -INFINITY;
-        const bool mine = v >= reach;
-        const unsigned who = __ballot_sync(0xffffffffu, mine);
+    for (int i0 = warp; i0 < listed; i0 += SEL_WARPS * SEL_AGAIN) {
+        float v[SEL_AGAIN];
+        int p[SEL_AGAIN], many = 0;
+#pragma unroll
+        for (int u = 0; u < SEL_AGAIN; ++u) {
+            const int i = i0 + u * SEL_WARPS, piece = i < listed ? pieces[i] : 0;
+            p[u] = lo + piece / SEL_THREADS * SEL_TILE + where(piece % SEL_THREADS, lane);
+            v[u] = i < listed && p[u] < hi ? row[p[u]] : -INFINITY;
+        }
+        unsigned who[SEL_AGAIN];
+#pragma unroll
+        for (int u = 0; u < SEL_AGAIN; ++u) who[u] = __ballot_sync(0xffffffffu, v[u] >= reach), many += __popc(who[u]);
         int to = 0;
-        if (lane == 0) to = atomicAdd(&taken, __popc(who));
-        to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1u));
-        if (mine && to < SEL_POOL) key[to] = finite_key(v), place[to] = p;
+        if (lane == 0) to = atomicAdd(&taken, many);
+        to = __shfl_sync(0xffffffffu, to, 0);
+#pragma unroll
+        for (int u = 0; u < SEL_AGAIN; ++u) {
+            const int at_u = to + __popc(who[u] & ((1u << lane) - 1u));
+            if (v[u] >= reach && at_u < SEL_POOL) key[at_u] = finite_key(v[u]), place[at_u] = p[u];
+            to += __popc(who[u]);
+        }
     }
     __syncthreads();
     const int found = taken;
@@ -230,12 +242,15 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(const float* 
     const size_t row0 = (size_t)blockIdx.x * width;
     heads += row0 * parts, best += row0 * parts * count, at += row0 * parts * count, scores += row0;
     const int per_row = parts * count, all = width * per_row;
-    // a thread's first candidates are asked for before the rows' sums are made, and kept
+    // A thread's candidates: one of each 512, at another rank of its list each time (the lists are in order: with the same rank throughout, a few threads would
+    // hold all the best, and their maxima would let through more than the pool takes: 128 wanted, 16 requests of 8 beams over 151,936 tokens, 141 us).
+    auto candidate = [&](int h) { return h * MERGE_THREADS + ((threadIdx.x + h * 197) & (MERGE_THREADS - 1)); };
+    // the first ones are asked for before the rows' sums are made, and kept
     int held_at[MERGE_HELD];
     float held_best[MERGE_HELD];
 #pragma unroll
     for (int h = 0; h < MERGE_HELD; ++h) {
-        const int i = h * MERGE_THREADS + threadIdx.x;
+        const int i = candidate(h);
         held_at[h] = i < all ? at[i] : -1, held_best[h] = i < all ? best[i] : 0.0f;
     }
     for (int b = warp; b < width; b += MERGE_WARPS) {
@@ -268,9 +283,12 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_merge_kernel(const float* 
     };
     auto each = [&](auto&& f) {                              // every candidate; the rows are spread over all threads
 #pragma unroll
-        for (int h = 0; h < MERGE_HELD; ++h) one(h * MERGE_THREADS + threadIdx.x, held_at[h], held_best[h], f);
+        for (int h = 0; h < MERGE_HELD; ++h) one(candidate(h), held_at[h], held_best[h], f);
 #pragma unroll 4
-        for (int i = MERGE_HELD * MERGE_THREADS + threadIdx.x; i < all; i += MERGE_THREADS) one(i, at[i], best[i], f);
+        for (int h = MERGE_HELD; h * MERGE_THREADS < all; ++h) {
+            const int i = candidate(h);
+            if (i < all) one(i, at[i], best[i], f);
+        }
     };
     unsigned long long mine = 0;
     int c = 0;
