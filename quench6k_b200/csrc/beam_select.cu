@@ -92,8 +92,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
     __shared__ int red[SEL_WARPS];
     __shared__ PartHead of_warp[SEL_WARPS];
     __shared__ unsigned slots[SEL_THREADS];
-    __shared__ unsigned key[SEL_POOL];
-    __shared__ int place[SEL_POOL];
+    __shared__ __align__(16) unsigned long long pool[SEL_POOL];      // a logit's key above the complement of its place: the order of the result in one number
     __shared__ float piece_most[SEL_TILES][SEL_THREADS];
     __shared__ unsigned short pieces[SEL_TILES * SEL_THREADS];
     __shared__ int taken, listed;
@@ -182,7 +181,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
 #pragma unroll
         for (int u = 0; u < SEL_AGAIN; ++u) {
             const int at_u = to + __popc(who[u] & ((1u << lane) - 1u));
-            if (v[u] >= reach && at_u < SEL_POOL) key[at_u] = finite_key(v[u]), place[at_u] = p[u];
+            if (v[u] >= reach && at_u < SEL_POOL) pool[at_u] = (unsigned long long)finite_key(v[u]) << 32 | (unsigned)~p[u];
             to += __popc(who[u]);
         }
     }
@@ -191,11 +190,10 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
     if (found <= SEL_POOL) {
         for (int i = threadIdx.x; i < found; i += SEL_THREADS) {
             int rank = 0;
-            const unsigned k = key[i];
-            const int p = place[i];
+            const unsigned long long k = pool[i];
 #pragma unroll 8
-            for (int j = 0; j < found; ++j) rank += key[j] > k || (key[j] == k && place[j] < p);
-            if (rank < count) best[rank] = key_value(k), at[rank] = p;
+            for (int j = 0; j < found; ++j) rank += pool[j] > k;
+            if (rank < count) best[rank] = key_value((unsigned)(k >> 32)), at[rank] = (int)~(unsigned)k;
         }
         for (int i = found + threadIdx.x; i < count; i += SEL_THREADS) at[i] = -1;
         return;
