@@ -2041,6 +2041,7 @@ def hyper_step(x: torch.Tensor, S: int, add=None, read=None, rows: Optional[torc
 
 # --------------------------------------------------------------------------- products in 8-bit integers
 # The launchers below are called with plain numbers (a ctypes object for each argument is what takes most of a short call's host time).
+# Sizes go to torch.empty one by one: as a tuple they take it 2.3 us, so 1.5.
 _p, _t = ctypes.c_void_p, ctypes.c_int
 _I8_OPERANDS = [_p, _ll, _p, _t, _p, _p, _p, _p, _t, _t, _p, _p, _t, _p, _t, _p, _ll, _t, _f, _t]
 _ARGTYPES.update({
@@ -2100,8 +2101,8 @@ def quantize_rows(x: torch.Tensor):
     R, K = x.shape
     if K < 1 or R >= 1 << 31 or K > 1 << 30:
         raise KernelError(f"quantize_rows: {R} rows of {K} values")
-    q = torch.empty((R, K), dtype=torch.int8, device=x.device)
-    scale = torch.empty((R,), dtype=torch.float32, device=x.device)
+    q = torch.empty(R, K, dtype=torch.int8, device=x.device)
+    scale = torch.empty(R, dtype=torch.float32, device=x.device)
     _call("q6k_quantize_rows", x.data_ptr(), pitch, R, K, code, q.data_ptr(), scale.data_ptr(), _stream_of(device), launches=1 if R else 0)
     return q, scale
 
@@ -2130,7 +2131,7 @@ def _i8_product(w, w_scale, w2, w2_scale, K: int, grouped: bool, accumulate: boo
     if out is None:
         if accumulate:
             raise KernelError(f"{who}: accumulate needs an output")
-        out = torch.empty((rows, N), dtype=dtype, device=w.device)
+        out = torch.empty(rows, N, dtype=dtype, device=w.device)
     elif out.dtype is not dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != N or not out.is_contiguous():
         raise KernelError(f"{who}: out is {out.dtype} {tuple(out.shape)}, needs contiguous {dtype} [{rows}, {N}]")
     return (shape[0] if grouped else 1), N, epi, out
@@ -2240,8 +2241,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int):
     if not 1 <= width <= BEAM_MAX_WIDTH or not 1 <= count <= min(BEAM_MAX_COUNT, width * V) or width * V >= 1 << 31 or rows > 65535:
         raise KernelError(f"beam_select: {count} continuations (1 to {BEAM_MAX_COUNT}) of {requests} requests of {width} beams (1 to {BEAM_MAX_WIDTH}) over {V} tokens")
     nbytes = _beam_scratch(rows, V, count) if rows else 0
-    out = torch.empty((requests, count), dtype=torch.float32, device=logits.device)
-    beams, tokens = torch.empty((2, requests, count), dtype=torch.int32, device=logits.device).unbind(0)
+    out = torch.empty(requests, count, dtype=torch.float32, device=logits.device)
+    beams, tokens = torch.empty(2, requests, count, dtype=torch.int32, device=logits.device).unbind(0)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
     _call("q6k_beam_select", logits.data_ptr(), scores.data_ptr(), requests, width, V, count, scratch.data_ptr(), nbytes, out.data_ptr(), beams.data_ptr(), tokens.data_ptr(),
           _stream_of(device), launches=2 if rows else 0)
