@@ -125,14 +125,16 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) beam_part_kernel(const float* 
         piece_most[t][threadIdx.x] = high;
         const float m = fmaxf(most, high);
         if (m > -INFINITY) {
-            // 2^(x L - c) with c = m L rounded: the rounding of c multiplies the whole sum by 2^d, d = m L - c, which is known exactly
+            // 2^(x L - c) with c = m L rounded: the rounding of c multiplies the whole sum by 2^d, d = m L - c, which is known exactly.  d is up to 2^-24 of c, so
+            // that 2^d and 2^-d leave the range of a float where c is beyond 2^31, and m L itself may be infinite: from |m| = 10^6 on (d up to 1/16) the
+            // differences x - m, which are exact there for every x whose term counts, are taken instead.
             const float c = m * LOG2E, d = fmaf(m, LOG2E, -c);
             float here = 0.0f;
-            if (fabsf(m) < 1e30f) {
+            if (fabsf(m) < 1e6f) {
 #pragma unroll
                 for (int j = 0; j < SEL_EACH; ++j) here += ex2_approx(fmaf(v[j], LOG2E, -c));
                 here *= ex2_approx(-d);
-            } else {                                         // m L may be infinite
+            } else {
 #pragma unroll
                 for (int j = 0; j < SEL_EACH; ++j) here += ex2_approx((v[j] - m) * LOG2E);
             }

@@ -121,6 +121,27 @@ def test_tokens_masked_with_the_lowest_value():
     check_select(-x[:1], np.array([[-1.0]], dtype=np.float32), 20)
 
 
+@pytest.mark.parametrize("mask", [-6.5e4, -9.9e5, -1e6, -1e9, -1e10, -1e12, -1e20, -9e29, -2e30])
+def test_tokens_masked_with_a_large_finite_value(mask):
+    """Masks of any size leave a row's sum and its other tokens as they are; threads, tiles and whole parts of a row see nothing but the mask."""
+    x = np.full((4, 30000), mask, dtype=np.float32)
+    keep = np.random.default_rng(11).permutation(30000)[:60]
+    x[:, keep] = logits_of(13, 4, 30000)[:, keep]
+    x[3] = logits_of(14, 1, 30000)[0]
+    x[3, 8192:] = mask
+    check_select(x, scores_of(15, 1, 4), 24)
+    check_select(x, scores_of(15, 2, 2), 24)
+    check_select(x[:1], np.array([[-1.0]], dtype=np.float32), 80)         # every token that is left, then masked ones in order of place
+
+
+@pytest.mark.parametrize("level", [1e6, 3e9, -1e10, 1e10, -1e15, 1e29])
+def test_rows_of_a_large_level(level):
+    """Logits that differ by whole steps of a large number: equal ones share the row, the others count for nothing."""
+    step = np.spacing(np.float32(abs(level)))
+    x = (np.float32(level) + np.random.default_rng(17).integers(-3, 1, (3, 9001)).astype(np.float32) * step * 64).astype(np.float32)
+    check_select(x, np.array([[-1.0, -2.5, -7.25]], dtype=np.float32), 32)
+
+
 @pytest.mark.parametrize("V", [70000, 70001])
 def test_rows_whose_logits_ascend_or_descend(V):
     """Orders that hide the best from a threshold of the first logits, or show them all at once."""
