@@ -250,7 +250,7 @@ void launch(const I8Args& p, int pairs, cudaStream_t st) {
 
 // Whether rows (not pairs) come here rather than to the tensor-memory kernel: up to eight, or sixteen against a matrix of less than 32 MB (16 rows: 2,048 x
 // 2,048 4.0 us here and 7.0 there, 5,120 x 2,048 7.1 and 9.0; 32,768 x 2,048 20 and 15, 151,936 x 2,048 64 and 52).
-bool few_rows(const I8Args& p) { return p.rows <= 8 || (p.rows <= R8_ROWS && (long long)p.N * p.K * (p.w2 ? 2 : 1) < (32LL << 20)); }
+bool few_rows(int rows, int N, int K, bool dual) { return rows <= 8 || (rows <= R8_ROWS && (long long)N * K * (dual ? 2 : 1) < (32LL << 20)); }
 
 // Columns and loads of a block.  Measured in a graph, weights from HBM (columns x loads a row; the first is taken):
 //   one matrix: 4 loads of 16 columns (8 rows, 32,768 x 2,048: 15.6 us, 2 x 32 columns 17.3; 151,936 x 2,048: 54, 61), 8 where rows are long and blocks few (2,048 x
@@ -289,14 +289,18 @@ int launch_rows(const I8Args& p, cudaStream_t st) {
 int q6k_quantize_rows_launch(const void* x, long long ldx, int R, int K, int dtype, void* q, float* scale, cudaStream_t st);
 int q6k_gemm_i8_tc_launch(const I8Args& p, int a_total, void* gathered, cudaStream_t st);
 
-// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered: rows * (K + 4) bytes of scratch, where a_rows comes with more than eight rows or with
-// groups.
+// Bytes of scratch that q6k_gemm_i8 takes for rows that are picked (a_rows), with groups or without; 0: the product reads them where they are.
+Q6K_API long long q6k_gemm_i8_scratch(int rows, int N, int K, int dual, int grouped) {
+    return !grouped && few_rows(rows, N, K, dual != 0) ? 0 : (long long)rows * (K + 4LL);
+}
+
+// See ops.gemm_i8 for the operands.  a has `a_total` rows.  gathered: scratch for rows that are picked, 16-byte aligned (q6k_gemm_i8_scratch).
 Q6K_API int q6k_gemm_i8(I8_OPERANDS, int a_total, void* gathered, cudaStream_t st) {
     I8Args p;
     if (int rc = i8_args(&p, "gemm_i8", I8_NAMES)) return rc;
     Q6K_REQUIRE(!pair_expert, "gemm_i8: pairs come with rows that are not in 8 bits");
     p.a_total = a_total;
-    if (!offsets && few_rows(p)) return launch_rows(p, st);
+    if (!offsets && few_rows(rows, N, K, w2 != nullptr)) return launch_rows(p, st);
     return q6k_gemm_i8_tc_launch(p, a_total, gathered, st);
 }
 
@@ -315,7 +319,7 @@ Q6K_API int q6k_linear_i8(const void* x, long long ldx, int T, int dtype, void* 
         return rc;
     Q6K_REQUIRE(!offsets && !a_rows && (pair_expert ? (rows + pair_div - 1) / pair_div <= T : rows == T), "linear_i8: %d rows of %d", rows, T);
     if (rows == 0) return 0;
-    const bool few = pair_expert || few_rows(p);
+    const bool few = pair_expert || few_rows(rows, N, K, w2 != nullptr);
     if (q6k_linear_i8_scratch(T, N, K, dtype, ((uintptr_t)x & 15) == 0, pair_expert != nullptr) == 0) {
         p.x = (const __nv_bfloat16*)x, p.early = early;
         const int blocks = (N + 15) / 16;

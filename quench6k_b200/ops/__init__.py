@@ -2141,6 +2141,13 @@ def _data(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=1024)          # a question about sizes: asked of the library once
+def _gemm_i8_scratch(rows: int, N: int, K: int, dual: bool, grouped: bool) -> int:
+    lib = library()
+    lib.q6k_gemm_i8_scratch.restype = ctypes.c_longlong
+    return lib.q6k_gemm_i8_scratch(_i(rows), _i(N), _i(K), _i(dual), _i(grouped))
+
+
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
             accumulate: bool = False, w2: Optional[torch.Tensor] = None, w2_scale: Optional[torch.Tensor] = None, act=None,
             offsets: Optional[torch.Tensor] = None, a_rows: Optional[torch.Tensor] = None, early: bool = False) -> torch.Tensor:
@@ -2171,8 +2178,9 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     if grouped:
         _is(offsets, "offsets", torch.int32, (groups + 1,))
     gathered = None                      # the rows that are picked, side by side, and their scales
-    if a_rows is not None and (grouped or rows > 8):
-        gathered = torch.empty(rows * (K + 4), dtype=torch.uint8, device=a.device)
+    if a_rows is not None:
+        nbytes = _gemm_i8_scratch(rows, N, K, w2 is not None, grouped)
+        gathered = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
     _call("q6k_gemm_i8", a.data_ptr(), lda, a_scale.data_ptr(), rows, w.data_ptr(), w_scale.data_ptr(), _data(w2), _data(w2_scale), N, K, _data(a_rows), _data(offsets),
           groups, 0, 1, out.data_ptr(), N, epi, _act_param(act), early, total, _data(gathered), _stream_of(device),
           launches=0 if rows == 0 else 1 if gathered is None else 2)

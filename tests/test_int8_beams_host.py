@@ -19,3 +19,13 @@ def test_operands_on_the_host_are_refused():
 def test_a_type_without_kernels_is_refused():
     with pytest.raises(ops.KernelError, match="float32 or bfloat16"):
         ops.quantize_rows(torch.zeros(4, 32, dtype=torch.float64))
+
+
+def test_scratch_for_picked_rows():
+    """Rows that the product of few rows reads where they are take none; others are brought side by side, with their scales."""
+    assert [ops._gemm_i8_scratch(rows, 100, 1024, False, False) for rows in (0, 1, 8, 9, 12, 16)] == [0] * 6
+    assert ops._gemm_i8_scratch(17, 100, 1024, False, False) == 17 * 1028
+    # sixteen rows against 32 MB of weights and more go to the tiles
+    assert ops._gemm_i8_scratch(12, 32768, 1024, False, False) == 12 * 1028 and ops._gemm_i8_scratch(12, 32767, 1024, False, False) == 0
+    assert ops._gemm_i8_scratch(12, 16384, 1024, True, False) == 12 * 1028 and ops._gemm_i8_scratch(8, 32768, 1024, True, False) == 0
+    assert ops._gemm_i8_scratch(3, 100, 1024, True, True) == 3 * 1028 and ops._gemm_i8_scratch(1 << 20, 100, 131056, False, True) == 131060 << 20

@@ -304,6 +304,20 @@ def test_rows_that_are_picked(rows, n):
     near(ops.gemm_i8(a.cuda(), s.cuda(), w.cuda(), t.cuda(), a_rows=pick.cuda()), product64(a[pick.long()], s[pick.long()], w, t), STORED)
 
 
+@pytest.mark.parametrize("rows,n,launches,scratch", [(8, 100, 1, 0), (9, 100, 1, 0), (16, 100, 1, 0), (17, 100, 2, 17 * 1028), (9, 33000, 2, 9 * 1028)])
+def test_picked_rows_take_the_launches_and_the_memory_that_are_counted(rows, n, launches, scratch, monkeypatch):
+    from quench6k_b200 import ops
+    a, s, ((w, t),) = operands(rows, 20, n, 1024)
+    a, s, w, t = a.cuda(), s.cuda(), w.cuda(), t.cuda()
+    pick = torch.randint(0, 20, (rows,), generator=torch.Generator().manual_seed(rows), dtype=torch.int32).cuda()
+    out = torch.empty(rows, n, device="cuda")
+    taken, empty = [], torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *size, **kw: (taken.append(size), empty(*size, **kw))[1])
+    before = ops.launch_count
+    ops.gemm_i8(a, s, w, t, out=out, a_rows=pick)
+    assert ops.launch_count - before == launches and taken == ([(scratch,)] if scratch else [])
+
+
 @pytest.mark.parametrize("rows,n", [(5, 100), (12, 33000), (40, 100)])
 def test_a_picked_row_that_is_none_is_a_row_of_nan(rows, n):
     from quench6k_b200 import ops
