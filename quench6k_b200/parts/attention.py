@@ -133,16 +133,11 @@ class Attention(Mixer):
 
     def bind(self, get, rt):
         self.rt = rt
-        # q, k and v rows stacked so one product yields [q | k | v] per token: each piece is copied into its place
-        # on the device as it arrives, so that no two copies of the three are held at once
+        # q, k and v rows stacked so one product yields [q | k | v] per token, and the heads' gates behind them
         nq, nk, nv, n = self.nq, self.nk, self.nv, self.names
         pieces = ("q", "k") if self.values_are_keys else ("q", "k", "v")
-        self.w_qkv = (torch.zeros if self.ng else torch.empty)((nq + nk + nv + self.ng, self.D), dtype=rt.dtype, device=rt.device)
-        if self.head_gate:
-            self.w_qkv[self.g_col:self.g_col + self.Hq].copy_(get(n["gate"]))
-        for name, lo, hi in ((n["q"], 0, nq), (n["k"], nq, nq + nk), (n["v"], nq + nk, nq + nk + nv))[:len(pieces)]:
-            self.w_qkv[lo:hi].copy_(get(name))
-        self.w_qkv = linear.to_weight(self.w_qkv, rt)
+        stack = list(zip((0, nq, nq + nk), pieces)) + ([(self.g_col, "gate")] if self.head_gate else [])
+        self.w_qkv = linear.stacked_weight(nq + nk + nv + self.ng, self.D, [(at, n[x]) for at, x in stack], get, rt)
         self.w_q = self.w_qkv if self.head_gate else self.w_qkv[:nq]      # what a layer that reads another's pages multiplies with
         self.w_o = linear.to_weight(get(n["o"]), rt)
         if self.qk_norm and self.qk_norm_weight:

@@ -43,12 +43,31 @@ def int8_rows_allowed(K: int) -> bool:
 
 def to_weight(t: torch.Tensor, rt):
     """A stored matrix as the products consume it: in the operand dtype, or in 8 bits where the runtime keeps its weights so and
-    the kernels take its rows."""
-    w = to_operand(t, rt)
-    if not rt.int8_weights or not int8_rows_allowed(w.shape[-1]):
-        return w
+    the kernels take its rows.  Those 8 bits are the only rounding: a matrix stored in 32 bits does not pass through the operand dtype."""
+    if not rt.int8_weights or not int8_rows_allowed(t.shape[-1]):
+        return to_operand(t, rt)
+    w = t.to(device=rt.device, dtype=t.dtype if t.dtype == torch.bfloat16 else torch.float32).contiguous()
     q, scale = ops.quantize_rows(w.view(-1, w.shape[-1]))
     return Int8Matrix(q.view(w.shape), scale.view(w.shape[:-1]))
+
+
+def stacked_weight(rows: int, K: int, pieces, get, rt):
+    """The same for one matrix [rows, K] of stored matrices, (first row, tensor name) each; rows that none of them covers are zeros.
+    The tensors are fetched and put in their places one by one, so that no two copies of all of them are held at once."""
+    if rt.int8_weights and int8_rows_allowed(K):
+        w = Int8Matrix(torch.zeros((rows, K), dtype=torch.int8, device=rt.device), torch.zeros(rows, dtype=torch.float32, device=rt.device))
+        for at, name in pieces:
+            part = to_weight(get(name), rt)
+            w.q[at:at + part.shape[0]].copy_(part.q)
+            w.scale[at:at + part.shape[0]].copy_(part.scale)
+            del part
+        return w
+    w = torch.zeros((rows, K), dtype=rt.dtype, device=rt.device)
+    for at, name in pieces:
+        part = get(name)
+        w[at:at + part.shape[0]].copy_(part)
+        del part
+    return w
 
 
 def matmul(a: torch.Tensor, w: torch.Tensor, rt, out: Optional[torch.Tensor] = None, accumulate: bool = False,

@@ -151,3 +151,56 @@ def test_what_is_refused(tmp_path):
         Engine.from_folder(str(tmp_path), dtype="float32", weights="int8")
     with pytest.raises(ValueError, match="int8"):
         Engine.from_folder(str(tmp_path), weights="int4")
+
+
+def in_32_bits(folder, config, helper):
+    """The model's folder again with its matrices stored in 32 bits; the stored tensors by name."""
+    import os
+    from quench6k_b200.weights.safetensors_io import write_safetensors
+    _, weights = helper(folder, config)
+    for i, (name, t) in enumerate(weights.items()):
+        if t.dtype == torch.bfloat16:
+            weights[name] = torch.randn(t.shape, generator=torch.Generator().manual_seed(i)) * 0.1
+    write_safetensors(os.path.join(folder, "model.safetensors"), weights.items())
+    return weights
+
+
+@pytest.mark.parametrize("name", ["flint_D", "gunenex"])
+def test_matrices_stored_in_32_bits_are_rounded_once(name, tmp_path):
+    """The 8 bits of every matrix are those of its stored values, not of their bfloat16 roundings."""
+    import gunenex_configs
+    import gunenex_helpers
+    from test_int8_gpu import quantized
+    from quench6k_b200.engine import ModelRunner
+    from quench6k_b200.parts.attention import Attention
+    from quench6k_b200.parts.linear import Int8Matrix
+    source = {"flint_D": lambda f: in_32_bits(f, "D", helpers.make_model_folder),
+              "gunenex": lambda f: in_32_bits(f, gunenex_configs.get("G1"), gunenex_helpers.make_folder)}[name](str(tmp_path))
+    model = ModelRunner.from_folder(str(tmp_path), num_pages=4, max_requests=2, weights="int8").model
+
+    def check(matrix, stored):
+        q, scale = quantized(stored.reshape(-1, stored.shape[-1]).numpy())
+        assert isinstance(matrix, Int8Matrix) and tuple(matrix.shape) == tuple(stored.shape)
+        assert torch.equal(matrix.q.cpu().view(q.shape), torch.from_numpy(q)) and torch.equal(matrix.scale.cpu().view(-1), torch.from_numpy(scale))
+
+    seen = 0
+    for spec, block in zip(model.spec.layers, model.blocks):
+        parts = [(spec.prefix + model.spec.sub_names[sub], part) for sub, part in block.parts()]
+        parts += [(pre + part.names[side], inner) for pre, part in parts if hasattr(part, "sides") for side, inner in part.sides.items()]
+        for pre, part in parts:
+            stored = lambda n: source[pre + n]
+            if isinstance(part, Attention):
+                rows = [stored(part.names[x]) for x in ("q", "k", "v") if not (x == "v" and part.values_are_keys)]
+                if part.head_gate:
+                    rows += [stored(part.names["gate"]), torch.zeros(part.ng - part.Hq, part.D)]
+                check(part.w_qkv, torch.cat(rows))
+                check(part.w_o, stored(part.names["o"]))
+                seen += 1
+            elif hasattr(part, "w_down"):
+                for attr, key in (("w_up", "up"), ("w_gate", "gate"), ("w_down", "down")):
+                    if isinstance(getattr(part, attr), Int8Matrix):        # (rows that are no multiple of 16 long stay as they are)
+                        check(getattr(part, attr), stored(part.names[key]))
+                        seen += 1
+    if model.spec.head_name is not None:
+        check(model.head, source[model.spec.head_name])
+    assert seen >= (8 if name == "flint_D" else 2)
