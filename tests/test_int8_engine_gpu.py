@@ -204,3 +204,94 @@ def test_matrices_stored_in_32_bits_are_rounded_once(name, tmp_path):
     if model.spec.head_name is not None:
         check(model.head, source[model.spec.head_name])
     assert seen >= (8 if name == "flint_D" else 2)
+
+
+def with_rows_in_8_bits(config):
+    """The configuration with feed-forwards whose widths the 8-bit products take."""
+    if isinstance(config, dict):
+        return {k: -(-v // 16) * 16 if k == "ff" else with_rows_in_8_bits(v) for k, v in config.items()}
+    return [with_rows_in_8_bits(v) for v in config] if isinstance(config, list) else config
+
+
+ROUTED = {
+    **{name: MODELS[name] for name in ("flint_D", "flint_B")},
+    "kipedra": lambda f: kipedra_helpers.make_folder(f, with_rows_in_8_bits(kipedra_configs.get("K1")), seed=7, init_std=0.08),
+    "kitodra": lambda f: kitodra_helpers.make_folder(f, with_rows_in_8_bits(kitodra_configs.get("T1")), seed=7, init_std=0.08),
+    "kodatar": lambda f: kodatar_helpers.make_folder(f, with_rows_in_8_bits(kodatar_configs.get("K1")), seed=7, init_std=0.08),
+}
+
+
+class Checked:
+    """ops.linear_i8 and ops.gemm_i8 whose every result is compared with the formula in 64 bits on the call's own operands; `seen`: how many
+    results of each form were."""
+
+    def __init__(self, ops, monkeypatch):
+        self.seen, self.quantize = {}, ops.quantize_rows
+        for name in ("linear_i8", "gemm_i8"):
+            real = getattr(ops, name)
+            monkeypatch.setattr(ops, name, lambda *a, _real=real, _f=getattr(self, name), **kw: _f(_real, *a, **kw))
+
+    def linear_i8(self, real, x, w, w_scale, out=None, accumulate=False, w2=None, w2_scale=None, act=None, pair_expert=None, pair_div=1, weights_are_old=False):
+        base = out.clone() if accumulate else None
+        y = real(x, w, w_scale, out=out, accumulate=accumulate, w2=w2, w2_scale=w2_scale, act=act, pair_expert=pair_expert, pair_div=pair_div, weights_are_old=weights_are_old)
+        q, s = self.quantize(x)
+        if pair_expert is None:
+            self.check("one row" if x.shape[0] == 1 else "rows", y, base, q, s, [(w, w_scale), (w2, w2_scale)], act)
+        else:
+            e = pair_expert.long()
+            row = torch.arange(e.numel(), device=x.device) // pair_div
+            self.groups("pairs", y, q[row], s[row], [e == g for g in range(w.shape[0])], w, w_scale, w2, w2_scale, act)
+        return y
+
+    def gemm_i8(self, real, a, a_scale, w, w_scale, w2=None, w2_scale=None, act=None, offsets=None, a_rows=None, early=False):
+        y = real(a, a_scale, w, w_scale, w2=w2, w2_scale=w2_scale, act=act, offsets=offsets, a_rows=a_rows, early=early)
+        if a_rows is not None:
+            a, a_scale = a[a_rows.long()], a_scale[a_rows.long()]
+        at = torch.arange(a.shape[0], device=a.device)
+        self.groups("grouped, picked" if a_rows is not None else "grouped", y, a, a_scale, [(at >= offsets[g]) & (at < offsets[g + 1]) for g in range(w.shape[0])],
+                    w, w_scale, w2, w2_scale, act)
+        return y
+
+    def groups(self, form, y, q, s, members, w, w_scale, w2, w2_scale, act):
+        for g, mine in enumerate(members):
+            self.check(form, y[mine], None, q[mine], s[mine], [(w[g], w_scale[g]), (w2, w2_scale) if w2 is None else (w2[g], w2_scale[g])], act)
+
+    def check(self, form, y, base, q, s, mats, act):
+        from test_int8_gpu import BF16_HALF, HALF, STORED, gated64, product64
+        if y.numel() == 0:
+            return
+        g = product64(q, s, *mats[0])
+        if mats[1][0] is None and act is None:
+            want, allowed = g if base is None else g + base.double(), STORED * g.abs()
+            if base is not None:
+                allowed = allowed + HALF * 1.01 * want.abs()
+        else:
+            u = torch.ones_like(g) if mats[1][0] is None else product64(q, s, *mats[1])
+            want = gated64(g, u, act)
+            # of the result: its rounding to bfloat16; three roundings of the gate's argument, which move silu by 1 + |g| times as much, and three of the other factor;
+            # an exponential off by 3 + 1.2 |g| units of two half steps; ten half steps of the gate's other arithmetic
+            allowed = want.abs() * (BF16_HALF * 1.01 + HALF * (3 * (1 + g.abs()) + 3 + 2 * (3 + 1.2 * g.abs()) + 10)) + 1e-30
+            if act not in (None, "silu"):          # sums that nearly cancel: a rounding counts in full
+                allowed = allowed + 8 * HALF * g.abs() * (u.abs() + 1)
+        off = (y.double() - want).abs()
+        assert bool((off <= allowed).all()), f"{form}, {tuple(y.shape)}, act {act}: off by {float((off / allowed).max()):.3g} of what is allowed"
+        self.seen[form] = self.seen.get(form, 0) + y.numel()
+
+
+@pytest.mark.parametrize("name", sorted(ROUTED))
+def test_every_product_of_a_models_steps(name, tmp_path, monkeypatch):
+    """Prompts, portions and single tokens: each product alone, so that a wrong one shows whatever the layers behind it make of it."""
+    import json
+    from quench6k_b200 import ops
+    from quench6k_b200.parts.ffn import RoutedExperts
+    ROUTED[name](str(tmp_path))
+    vocab = json.load(open(tmp_path / "config.json"))
+    vocab = vocab.get("vocab_size") or vocab["vocab"]
+    checked = Checked(ops, monkeypatch)
+    got, runner = logits_of(tmp_path, {"a": helpers.random_tokens(45, vocab, 2), "b": helpers.random_tokens(29, vocab, 3)}, cuda_graphs=False)
+    experts = [part for b in runner.model.blocks for _, part in b.parts() if isinstance(part, RoutedExperts)]
+    assert experts and all(part.int8 for part in experts)
+    # pair by pair where a part hands its rows on unsummed: not where it has a shared expert's to add to them (all layers of flint_B)
+    forms = {"one row", "rows", "grouped, picked", "grouped"} | ({"pairs"} if any(part.shared is None for part in experts) else set())
+    assert set(checked.seen) >= forms, checked.seen
+    assert bool(torch.isfinite(got).all()) and ops.tc_status() == 0
