@@ -367,8 +367,6 @@ int row_parts(long long rows, int V) {
 
 }  // namespace
 
-Q6K_API int q6k_beam_max_count() { return SEL_MAX_COUNT; }
-Q6K_API int q6k_beam_max_width() { return SEL_MAX_WIDTH; }
 // Bytes of scratch that q6k_beam_select takes.
 Q6K_API long long q6k_beam_scratch(int rows, int V, int count) {
     return (long long)rows * row_parts(rows, V) * ((long long)count * 8 + (long long)sizeof(PartHead));

@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(R8_WARPS * 32) gemm_i8_rows_kernel(const I8Arg
 }
 
 // Pairs against short rows: a warp takes 16 columns over all of K, so that nothing waits for another warp.  grid (blocks of 16 PAIR_WARPS columns, pairs).
+// The rows are taken to 8 bits by the launch in front, which has waited for all that is older: weights and pair list are fetched before the wait.
 constexpr int PAIR_WARPS = 4;
 template <bool DUAL, int LOADS>
 __global__ void __launch_bounds__(PAIR_WARPS * 32) gemm_i8_pairs_kernel(const I8Args p) {
@@ -193,10 +194,9 @@ __global__ void __launch_bounds__(PAIR_WARPS * 32) gemm_i8_pairs_kernel(const I8
     constexpr int MATS = DUAL ? 2 : 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, pair = lane & 3;
     const int n0 = (blockIdx.x * PAIR_WARPS + warp) * 16, row = blockIdx.y;
-    if (!p.early) pdl_wait();
     const int g = p.pair_expert[row];
     if ((unsigned)g >= (unsigned)p.groups || n0 >= p.N) {
-        if (p.early) pdl_wait();                          // a warp that ends has waited too: who waits for this kernel counts on it
+        pdl_wait();                                       // a warp that ends has waited too: who waits for this kernel counts on it
         return;
     }
     const uint64_t once = l2_evict_first_policy();
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(PAIR_WARPS * 32) gemm_i8_pairs_kernel(const I8
 #pragma unroll
                 for (int h = 0; h < 2; ++h) w[m][h][j] = k0 + j * 64 + pair * 16 < p.K ? ld_once(wrow[m][h] + k0 + j * 64, once) : make_uint4(0, 0, 0, 0);
         if (k0 == 0) {
-            if (p.early) pdl_wait();
+            pdl_wait();
             xs = p.a_scale[from];
         }
 #pragma unroll
@@ -269,9 +269,9 @@ int launch_rows(const I8Args& p, cudaStream_t st) {
     const bool deep = p.K >= 8192 && blocks < 4 * 148;
     if (p.pair_expert && (!p.w2 || p.K <= 256 || (p.K <= 2048 && blocks >= (p.K <= 1024 ? 5 : 8) * 148))) {
         const dim3 grid((p.N + PAIR_WARPS * 16 - 1) / (PAIR_WARPS * 16), pairs);
-        if (p.w2) q6k_launch_as(p.early != 0, gemm_i8_pairs_kernel<true, 4>, grid, PAIR_WARPS * 32, 0, st, p);
-        else if (p.K <= 256) q6k_launch_as(p.early != 0, gemm_i8_pairs_kernel<false, 4>, grid, PAIR_WARPS * 32, 0, st, p);
-        else q6k_launch_as(p.early != 0, gemm_i8_pairs_kernel<false, 8>, grid, PAIR_WARPS * 32, 0, st, p);
+        if (p.w2) q6k_launch_as(true, gemm_i8_pairs_kernel<true, 4>, grid, PAIR_WARPS * 32, 0, st, p);
+        else if (p.K <= 256) q6k_launch_as(true, gemm_i8_pairs_kernel<false, 4>, grid, PAIR_WARPS * 32, 0, st, p);
+        else q6k_launch_as(true, gemm_i8_pairs_kernel<false, 8>, grid, PAIR_WARPS * 32, 0, st, p);
     } else if (p.w2) {
         if (two == 2) launch<true, 2, 1, 4>(p, pairs, st);
         else if (p.pair_expert || blocks >= 4 * 148) launch<true, 1, 2, 2>(p, pairs, st);
@@ -310,8 +310,9 @@ Q6K_API long long q6k_linear_i8_scratch(int T, int N, int K, int dtype, int alig
     return T == 1 && !pairs && dtype == Q6K_BF16 && aligned && K <= 8192 && (N + 15) / 16 <= 2 * 148 ? 0 : (long long)T * K + 4LL * T;
 }
 
-// See ops.linear_i8: x of dtype code, T rows of pitch ldx; a, lda and a_scale of the operands are not looked at, and `early` says that the weights and
-// the pair list are older than the kernel before this call.  scratch: 16-byte aligned.
+// See ops.linear_i8: x of dtype code, T rows of pitch ldx; a, lda and a_scale of the operands are not looked at, and `early` says that the weights are
+// older than the kernel before this call, where the row is taken to 8 bits by the product (a launch of its own in front has waited for all that
+// is older).  scratch: 16-byte aligned.
 Q6K_API int q6k_linear_i8(const void* x, long long ldx, int T, int dtype, void* scratch, I8_OPERANDS, cudaStream_t st) {
     I8Args p;
     if (int rc = i8_args(&p, "linear_i8", scratch, K, (const float*)((char*)scratch + (long long)T * K), rows, w, w_scale, w2, w2_scale, N, K, a_rows, offsets, groups, pair_expert,

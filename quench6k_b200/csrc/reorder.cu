@@ -150,9 +150,6 @@ void launch_slots(const SlotTensors& t, int n, int groups, int width, int blocks
 
 }  // namespace
 
-Q6K_API int q6k_reorder_max_width() { return RE_MAX_WIDTH; }
-Q6K_API int q6k_reorder_max_tensors() { return RE_TENSORS; }
-
 // bases, heads, pages, row_bytes: n tensors [heads, pages, page_size, row_bytes] on the host's side; table: int32 [groups * width, blocks];
 // parents: int32 [groups, width]; first, lengths: int32 [groups * width].  Row r takes over positions first[r] .. lengths[parent] - 1.
 Q6K_API int q6k_reorder_pages(int n, const long long* bases, const int* heads, const int* pages, const int* row_bytes, const int* table, int groups, int width,

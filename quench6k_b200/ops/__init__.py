@@ -2158,8 +2158,8 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     act alone act(y); both leave in bfloat16.
     a_rows (int32 [rows]): row r of the product is row a_rows[r] of a (a number outside a: a row of NaN).  offsets (int32 [G + 1], ascending from 0) with w [G, N, K]
     and w_scale [G, N]: rows offsets[g] .. offsets[g + 1] - 1 go against matrix g; rows behind the last offset are left as they were.
-    early: the caller's word that the kernel before this call made a and a_scale and nothing else that is read here: the weights
-    are then fetched while it ends."""
+    early: the caller's word that the kernel before this call made a and a_scale, is no product (quantize_rows), and made nothing else that is read
+    here: the weights are then fetched while it ends."""
     if a.dtype is not torch.int8:
         raise KernelError(f"a has dtype {a.dtype}, expected torch.int8")
     grouped = offsets is not None
@@ -2200,9 +2200,10 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out: Opti
     """The product of quantize_rows(x) with weights in 8 bits: x float32 or bfloat16 [T, K] (its rows may lie apart), the rest as in
     gemm_i8.  With pair_expert (int32 [pairs], at most 65,535) and w [experts, N, K]: row y of the result is row y // pair_div of x
     against the matrix of expert pair_expert[y]; a pair that names no matrix is left as it was.
-    weights_are_old: the caller's word that the weights and the pair list were written before the kernel that precedes this call
-    on the stream started: they may then be fetched while it ends (a model's weights; they are not, if the call follows the
-    kernel that made them)."""
+    weights_are_old: the caller's word that the weights are older than the kernel that precedes this call on the stream, and not by products alone
+    (a model's weights): one row's product, a single launch, may then fetch them while that kernel ends.  Products start before the kernels in front
+    of them have ended, so behind the kernel that makes the weights there has to be a synchronisation or a kernel that is no product.  More
+    rows, and pairs, are taken to 8 bits by a launch in front, which waits for all that is older: there it changes nothing."""
     code = dtype_code(x.dtype)
     operands = [("x", x), ("w", w), ("w_scale", w_scale)]
     operands += [(n, t) for n, t in (("w2", w2), ("w2_scale", w2_scale), ("out", out), ("pair_expert", pair_expert)) if t is not None]

@@ -242,7 +242,7 @@ class RoutedExperts(FeedForward):
             act = self.act if not self.gated or self.act != "silu" else None
             first = linear.pair_products(xn, sel_e, self.k, self.w_gate, self.w_up if self.gated else None, act)     # [pairs, I]
             ops.current_tag = "experts.down"
-            return self._rows(linear.pair_products(first, sel_e, 1, self.w_down, pairs_are_old=True), sel_w, None, xn, more)
+            return self._rows(linear.pair_products(first, sel_e, 1, self.w_down), sel_w, None, xn, more)
         if (not self.int8 and T <= self.pair_tokens and defer and rt.tensor_cores and not rt.is_fp32 and ops.tc_supported(xn, self.w_up) and self.I % 8 == 0):
             # a step of a few tokens whose router is not the one-launch kernel's: still one weight tile stream per
             # (token, slot) pair straight from the selection, no permutation and no gather

@@ -191,13 +191,11 @@ def _uniform_groups(groups: int, rows_per_group: int, bm: int, device):
     return _uniform[key]
 
 
-def pair_products(a: torch.Tensor, sel_e: torch.Tensor, per_row: int, w: "Int8Matrix", w_up: Optional["Int8Matrix"] = None, act=None,
-                  pairs_are_old: bool = False) -> torch.Tensor:
+def pair_products(a: torch.Tensor, sel_e: torch.Tensor, per_row: int, w: "Int8Matrix", w_up: Optional["Int8Matrix"] = None, act=None) -> torch.Tensor:
     """A step of few tokens: y[p] = a[p // per_row] @ w_e^T for the expert e of pair p, FP32 (or act of it, or the gated form with
-    w_up, in bfloat16), straight from the selection.  pairs_are_old: the kernel before this call did not make the selection."""
+    w_up, in bfloat16), straight from the selection."""
     more = {} if w_up is None else {"w2": w_up.q, "w2_scale": w_up.scale}
-    return ops.linear_i8(a, w.q, w.scale, act=act, pair_expert=sel_e.view(-1), pair_div=per_row,
-                         weights_are_old=pairs_are_old, **more)
+    return ops.linear_i8(a, w.q, w.scale, act=act, pair_expert=sel_e.view(-1), pair_div=per_row, **more)
 
 
 def batched_matmul(a: torch.Tensor, w: torch.Tensor, rt, rows_per_group: int, rounded: bool = False) -> torch.Tensor:
