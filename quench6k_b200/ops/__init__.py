@@ -2328,7 +2328,7 @@ def reorder_pages(pages, table: torch.Tensor, parents: torch.Tensor, first: torc
     _is(table, "table", torch.int32, (rows, table.shape[1]))
     for n, *args in _batches(pages.args):
         _call("q6k_reorder_pages", n, *args, table.data_ptr(), groups, width, table.shape[1], pages.page_size, parents.data_ptr(), first.data_ptr(), lengths.data_ptr(),
-              _stream_of(device))
+              _stream_of(device), launches=1 if rows and table.shape[1] else 0)
 
 
 def reorder_slots(states, slots: torch.Tensor, parents: torch.Tensor) -> None:
@@ -2342,4 +2342,4 @@ def reorder_slots(states, slots: torch.Tensor, parents: torch.Tensor) -> None:
     if states.device.index != device:
         raise KernelError(f"reorder_slots: states on {states.device}, the current device is cuda:{device}")
     for n, *args in _batches(states.args):
-        _call("q6k_reorder_slots", n, *args, slots.data_ptr(), groups, width, parents.data_ptr(), _stream_of(device))
+        _call("q6k_reorder_slots", n, *args, slots.data_ptr(), groups, width, parents.data_ptr(), _stream_of(device), launches=1 if groups else 0)

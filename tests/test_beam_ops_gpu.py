@@ -347,3 +347,17 @@ def test_refusals():
         with pytest.raises(ops.KernelError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_reorderings_of_nothing_count_no_launch():
+    from quench6k_b200 import ops
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")
+    pages, states = [torch.ones(2, 3, 4, 8, device="cuda")], [torch.ones(5, 8, device="cuda")]
+    before = ops.launch_count
+    ops.reorder_pages(pages, i32(0, 3), i32(0, 2), i32(0), i32(0))
+    ops.reorder_pages(pages, i32(2, 0), i32(1, 2), i32(2), i32(2))
+    ops.reorder_slots(states, i32(0), i32(0, 2))
+    assert ops.launch_count == before and bool((pages[0] == 1).all()) and bool((states[0] == 1).all())
+    ops.reorder_pages(pages, i32(2, 3), i32(1, 2), i32(2), i32(2))
+    ops.reorder_slots(states, torch.arange(2, dtype=torch.int32, device="cuda"), i32(1, 2))
+    assert ops.launch_count == before + 2
