@@ -5,8 +5,9 @@
 //
 // Logits are read once.  A block takes a part of one row and leaves the part's maximum, its sum of exponentials over that
 // maximum, and its `count` best logits (within a row the order of the logits is the order of t).  A block per request then
-// makes the rows' sums and finds the best of what the parts left.  t is compared in 64 bits: two logits of one row that differ
-// give scores that differ, and scores of different beams are not made equal by a rounding.
+// makes the rows' sums and finds the best of what the parts left.  t is compared in 64 bits, where scores of different beams are not made equal by
+// a rounding to 32, nor those of logits of one row that differ by more than some 2^-52 of the score (closer ones, next to zero, are cut by the logit and
+// listed by place).
 #include <cfloat>
 
 #include "umma.cuh"

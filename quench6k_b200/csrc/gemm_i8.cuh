@@ -43,8 +43,9 @@ inline int i8_args(I8Args* p, const char* who, I8_OPERANDS) {
 // kernel writes, it may be these very weights, just taken to 8 bits.
 inline bool i8_overlaps(const I8Args& p) { return p.early != 0 && q6k_pdl_mode() != 0; }
 
-// silu(g) u by a fast quotient: it is off by some 2^-21 of the value, and the result is rounded to bfloat16 (2^-8); where e^-g is beyond 2^126 the value
-// is below 1e-36 and comes out as zero.
+// silu(g) u by a fast exponential and quotient: the exponential is off by up to 2 + 1.2 |g| units of 2^-23, which is the result's error where it outweighs the 1
+// (2^-17 at g = -40), the quotient by two; the result is then rounded to bfloat16 (2^-8).  Where e^-g is beyond 2^126 the value is below 1e-36 |u| and
+// comes out as zero.
 __device__ __forceinline__ float i8_silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 __device__ __forceinline__ float i8_gated(float g, float u, int act, float param) { return act == 0 ? i8_silu_times(g, u) : q6k_gated(g, u, act, param); }
 

@@ -31,6 +31,10 @@ __device__ __forceinline__ int parent_of(const int* parents, int group, int widt
 // so that which bytes a row takes over are two numbers.  grid (blocks along the pieces, tensors, groups); V: what a lane moves at a time; W: the most rows
 // of a group; U: places that a lane has under way at once.
 // (A thread for each place, which found its page and row by divisions of its own, held 150 registers: 163 us for 262 MB where this takes 60.)
+// What a row's pointers, bounds and values take in registers shows in wide groups: with 16 bytes at a time, 8 rows spill 156 bytes under the 80 registers
+// that let three blocks run, 16 take 248 registers and one block an SM, 32 spill 860 bytes.  1,024 positions in 48 tensors, half of the rows moving,
+// 805 MB (123 us at the copy's rate): groups of four 133 us, of eight 153, of sixteen 163; of 32 (512 positions) 182.  Three rows of five, 1,007 MB, 351 (154 at
+// the copy's rate): few loads under way in the form for eight.
 template <typename V, int W, int U>
 __global__ void __launch_bounds__(RE_THREADS, W <= 8 ? 3 : 1) reorder_pages_kernel(const __grid_constant__ PageTensors t, const int* table, int blocks, int page_size, const int* parents,
                                                                    const int* first, const int* lengths, int width) {
@@ -168,9 +172,9 @@ Q6K_API int q6k_reorder_pages(int n, const long long* bases, const int* heads, c
         if (pieces > most) most = pieces;
     }
     const int vb = vector_bytes(all);
-    // Enough blocks for every piece of the table, and no more than some eight to an SM in all (three run at a time): how many positions move is known on
-    // the device only, and a block without any costs its start (48 tensors, eight requests of four beams, 21 positions of 1,789: 12.7 us with sixteen, 9.7
-    // with eight, 7.8 with four; but all of 4,096 positions of two requests: 197, 199 and 214 us).
+    // Enough blocks for every piece of the table, and no more than some eight to an SM in all (three run at a time): first and lengths lie in device memory and
+    // the call says nothing else of how many positions move, and a block without any costs its start (48 tensors, eight requests of four beams, 21
+    // positions of 1,789: 12.7 us with sixteen, 9.7 with eight, 7.8 with four; but all of 4,096 positions of two requests: 197, 199 and 214 us).
     const long long want = (most + RE_THREADS / 32 - 1) / (RE_THREADS / 32), cap = (148 * 8 + (long long)n * groups - 1) / ((long long)n * groups);
     const int bx = (int)(want < cap ? want : cap);
     if (vb == 16) launch_pages<uint4>(t, n, groups, width, bx, table, blocks, page_size, parents, first, lengths, st);

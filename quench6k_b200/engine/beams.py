@@ -1,6 +1,7 @@
 """Beam search above the step function.
 
-A prompt runs once; its cache and states are then taken over by the other beams.  Every further step runs one token of each beam
+A prompt runs once; its cache and states are then copied to the other beams (a page has one owner: a search holds a prompt's pages once for
+each of its beams).  Every further step runs one token of each beam
 of all prompts as one batch (a decode step like any other: it replays the recording of its size), chooses the best continuations
 of each prompt on the device (ops.beam_select), and lets the beams that die go on from ones that live (ModelRunner.reorder): only
 the positions since the two parted are copied.  A beam that lives stays where it is.

@@ -33,8 +33,10 @@ def parse_dtype(d) -> torch.dtype:
 
 
 def make_runtime(device, dtype, tensor_cores: bool = True, weights: Optional[str] = None) -> Runtime:
-    """weights: None (the matrices in the operand dtype), or "int8" (bfloat16 only): the projections of attention, the dense and
-    routed feed-forwards and an untied LM head are kept in 8 bits with a scale for each output channel."""
+    """weights: None (the matrices in the operand dtype), or "int8" (bfloat16 only): the projections of attention over keys and values, the
+    dense and routed feed-forwards and an untied LM head are kept in 8 bits with a scale for each output channel, where their rows are a
+    multiple of 16 long.  Everything else stays in bfloat16: latent attention, the mixers without softmax attention, routers, embeddings (and a head
+    tied to them)."""
     if weights not in (None, "int8"):
         raise ValueError(f"weights {weights!r}: None or 'int8'")
     rt = Runtime(torch.device(device), parse_dtype(dtype), tensor_cores, weights == "int8")
